@@ -7,9 +7,10 @@
 ``batch``     small-batch decode: B sequences through one pass of B rows; btb's rows layout (forks of a shared prefix)
 ``session``   btb's session surface over an engine: feed / mark / rewind / crop / generate
 ``paged``     the paged cache with a shared-prefix tree
+``evict``     decoding over a cache of fixed size: the rows given least attention leave when it is full
 ``parallel``  one dense model tensor-parallel over the GPUs of a box; ``exchange`` its peer-mapped memory
 ``draft``     n-gram drafting and the speculative greedy loop; ``sampling`` the sampled pick's host side
 ``pack12``    btb's 12-bit lossless bf16 store, encoded on the card
 """
 
-__all__ = ["capi", "launcher", "engine", "moe", "batch", "session", "paged", "parallel", "exchange", "draft", "sampling", "pack12"]
+__all__ = ["capi", "launcher", "engine", "moe", "batch", "session", "paged", "evict", "parallel", "exchange", "draft", "sampling", "pack12"]

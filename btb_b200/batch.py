@@ -132,10 +132,15 @@ class RowsEngine(CardEngine):
     rows as B sequences of one token each in ONE cache - the forks of a prompt, which share its rows as their prefix, or a
     batch of prompts lying end to end - each row at its own position. Row b's keys are its prefix (`len` cache rows from
     `off`) and then its own steps, step i at cache row base + i * W + col, every row's step i in one stretch of W rows.
-    A row reads its keys in logical order, so its bits are its own one-sequence decode's whatever rows step beside it."""
+    A row reads its keys in logical order, so its bits are its own one-sequence decode's whatever rows step beside it.
 
-    def __init__(self, weights: ModelWeights, cap: int = 4096, device: Any = "cuda"):
+    `shared`: the attention goes over a prefix that several rows share once for all of them (`btb_b200_attn_shared`)
+    instead of once a row. A row then agrees with its own decode to rounding, not to the bit."""
+
+    def __init__(self, weights: ModelWeights, cap: int = 4096, device: Any = "cuda", shared: bool = False):
         super().__init__(weights, cap=cap, step_kernel=False, device=device)
+        self.shared = bool(shared)
+        self._shared_ws: Any = None
         self.rw = torch.zeros(3 + 3 * 32, dtype=torch.int32, device=self.dev)
         self.B = 0
         self._rows = False
@@ -191,6 +196,13 @@ class RowsEngine(CardEngine):
         M = pad_rows(T)
         self._k("btb_b200_norm_rope_kv_rows", ptr(g["qkv"]), ptr(wq), ptr(wk), c.eps, ptr(self.cos), ptr(self.sin),
                 ptr(self.rw), ptr(self.K[i]), ptr(self.V[i]), ptr(g["q"]), M, Hq, Hk, D, self.hs, self.rs, 0, self.cap, s)
+        if self.shared:
+            if self._shared_ws is None:  # sized for the widest pass: one workspace for every width's graph
+                n = int(capi.lib().btb_b200_attn_shared_workspace_bytes(32, Hq, Hk, D))
+                self._shared_ws = torch.empty(n, dtype=torch.uint8, device=self.dev)
+            self._k("btb_b200_attn_shared", ptr(g["q"]), ptr(self.K[i]), ptr(self.V[i]), ptr(out), ptr(self.rw), M, Hq, Hk,
+                    D, self.hs, self.rs, float(D**-0.5), ptr(self._shared_ws), win, ptr(sinks), self.cap, s)  # fmt: skip
+            return
         self._k("btb_b200_attn_decode_rows", ptr(g["q"]), ptr(self.K[i]), ptr(self.V[i]), ptr(out), ptr(self.rw), M, Hq,
                 Hk, D, self.hs, self.rs, float(D**-0.5), ptr(g["part_m"]), ptr(g["part_l"]), ptr(g["part_acc"]),
                 ptr(g["cnt"]), win, ptr(sinks), self.cap, s)  # fmt: skip

@@ -65,6 +65,9 @@ SIGNATURES: dict[str, tuple[Any, list[Any]]] = {
     "btb_b200_add_rmsnorm_wide": (_I, [_P, _P, _P, _F, _P, _P, _I, _I, _I, _P]),
     "btb_b200_silu_mul": (_I, [_P, _P, _I, _I, _P]),
     "btb_b200_norm_rope_kv": (_I, [_P, _P, _P, _F, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _LL, _LL, _I, _P, _I, _P]),
+    "btb_b200_norm_rope_kv_pos": (
+        _I, [_P, _P, _P, _F, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _LL, _LL, _I, _P, _I, _I, _P],
+    ),
     "btb_b200_norm_rope_kv_rows": (_I, [_P, _P, _P, _F, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _LL, _LL, _I, _I, _P]),
     "btb_b200_attn_decode_rows": (_I, [_P, _P, _P, _P, _P, _I, _I, _I, _I, _LL, _LL, _F, _P, _P, _P, _P, _I, _P, _I, _P]),
     "btb_b200_attn_decode": (
@@ -82,6 +85,16 @@ SIGNATURES: dict[str, tuple[Any, list[Any]]] = {
         _I, [_P, _P, _P, _F, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _LL, _LL, _I, _F, _P, _P, _P, _P, _I, _P, _I,
              _P, _P, _I, _P, _P],
     ),
+    "btb_b200_attn_shared": (_I, [_P, _P, _P, _P, _P, _I, _I, _I, _I, _LL, _LL, _F, _P, _I, _P, _I, _P]),
+    "btb_b200_attn_shared_workspace_bytes": (_SZ, [_I, _I, _I, _I]),
+    "btb_b200_attn_scored": (
+        _I, [_P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _LL, _LL, _F, _P, _LL, _P, _P, _P, _I, _P],
+    ),
+    "btb_b200_attn_scored_workspace_bytes": (_SZ, [_I, _I, _I, _I, _I]),
+    "btb_b200_kv_evict": (
+        _I, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _I, _LL, _LL, _I, _I, _LL, _LL, _I, _I, _I, _I, _P, _P, _P, _P],
+    ),
+    "btb_b200_kv_evict_workspace_bytes": (_SZ, [_I, _I, _I]),
     "btb_b200_attn_scratch_floats": (_SZ, [_I, _I, _I, _I]),
     "btb_b200_argmax_bf16": (_I, [_P, _I, _I, _P, _P, _P]),
     "btb_b200_argmax_scratch_bytes": (_SZ, [_I]),

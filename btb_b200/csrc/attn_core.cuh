@@ -336,6 +336,7 @@ struct RopeArgs {
     int T, Hq, Hk, centered;
     long long hs, rs;
     int cap;  // cache rows: a slot at or past it is refused
+    int positions = 0;  // rows of the cos/sin tables where positions are counted apart from cache rows, 0: cap
 };
 // the E values lane `lane` owns of `head` for row t at position `pos`: q and k heads normalised and rotated, a v head
 // as it stands - the bf16 values the cache and the query buffer hold
@@ -411,7 +412,7 @@ __device__ __forceinline__ void rope_item(const RopeArgs& A, int head, int t, in
         slot = n0 + t;
         pos = n0 + A.depth[t];
     }
-    if (slot < 0 || slot >= A.cap || pos < 0 || pos >= A.cap) {
+    if (slot < 0 || slot >= A.cap || pos < 0 || pos >= (A.positions > 0 ? A.positions : A.cap)) {
         if (lane == 0) b2_fail(B2_ERR_DOMAIN);
         return;
     }

@@ -340,7 +340,7 @@ extern "C" int btb_b200_silu_mul(const void* gu, void* m, int T, int I, void* st
 static int norm_rope_kv_impl(const void* qkv, const void* wq, const void* wk, float eps, const void* cos_t,
                              const void* sin_t, const void* n0p, const void* depth, const void* rw, void* K, void* V,
                              void* q, int T, int Hq, int Hk, int D, long long hs, long long rs, int centered,
-                             const void* tbl, int cap, void* stream) {
+                             const void* tbl, int cap, void* stream, int positions = 0) {
     if (!qkv || !cos_t || !sin_t || (!rw && (!n0p || !depth)) || !K || !V || !q) return B2_ERR_NULL;
     if (T <= 0 || Hq <= 0 || Hk <= 0 || cap <= 0) return B2_ERR_DOMAIN;
     // a lane reads its D/32 elements of a head, a norm weight or a table row as one load
@@ -352,7 +352,8 @@ static int norm_rope_kv_impl(const void* qkv, const void* wq, const void* wk, fl
     RopeArgs a{static_cast<const bf16*>(qkv), static_cast<const bf16*>(wq), static_cast<const bf16*>(wk),
                static_cast<const bf16*>(cos_t), static_cast<const bf16*>(sin_t), static_cast<const int*>(n0p),
                static_cast<const int*>(depth), static_cast<const int*>(tbl), static_cast<const int*>(rw),
-               static_cast<bf16*>(K), static_cast<bf16*>(V), static_cast<bf16*>(q), eps, T, Hq, Hk, centered, hs, rs, cap};
+               static_cast<bf16*>(K), static_cast<bf16*>(V), static_cast<bf16*>(q), eps, T, Hq, Hk, centered, hs, rs, cap,
+               positions};
     const dim3 grid(Hq + 2 * Hk, T);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     switch (D) {
@@ -369,6 +370,16 @@ extern "C" int btb_b200_norm_rope_kv(const void* qkv, const void* wq, const void
                                      const void* tbl, int cap, void* stream) {
     return norm_rope_kv_impl(qkv, wq, wk, eps, cos_t, sin_t, n0p, depth, nullptr, K, V, q, T, Hq, Hk, D, hs, rs, centered,
                              tbl, cap, stream);
+}
+
+// a cache that rows have left: the row of pass row t is still n0 + t, its position n0 + depth[t] may lie past the cache
+extern "C" int btb_b200_norm_rope_kv_pos(const void* qkv, const void* wq, const void* wk, float eps, const void* cos_t,
+                                         const void* sin_t, const void* n0p, const void* depth, void* K, void* V, void* q,
+                                         int T, int Hq, int Hk, int D, long long hs, long long rs, int centered,
+                                         const void* tbl, int cap, int positions, void* stream) {
+    if (positions <= 0) return B2_ERR_DOMAIN;
+    return norm_rope_kv_impl(qkv, wq, wk, eps, cos_t, sin_t, n0p, depth, nullptr, K, V, q, T, Hq, Hk, D, hs, rs, centered,
+                             tbl, cap, stream, positions);
 }
 
 // the rows layout: row t a sequence of its own, its token at position len + step, written to its step's cache row

@@ -155,6 +155,12 @@ int btb_b200_norm_rope_kv(const void* qkv, const void* wq, const void* wk, float
                           const void* sin_t, const void* n0p, const void* depth, void* K, void* V, void* q, int T,
                           int Hq, int Hk, int D, long long hs, long long rs, int centered, const void* tbl, int cap,
                           void* stream);
+/* btb_b200_norm_rope_kv over a cache that rows have been evicted from: positions and cache rows part, so the tables have
+ * `positions` rows of their own; a position n0 + depth[t] past them, or a row n0 + t past cap, is refused. */
+int btb_b200_norm_rope_kv_pos(const void* qkv, const void* wq, const void* wk, float eps, const void* cos_t,
+                              const void* sin_t, const void* n0p, const void* depth, void* K, void* V, void* q, int T,
+                              int Hq, int Hk, int D, long long hs, long long rs, int centered, const void* tbl, int cap,
+                              int positions, void* stream);
 /* btb_norm_rope_kv_rows_d{64,128,256} (btb_kernels.cu:228-248, 258-327 ROWS): the rows layout - a pass's T rows as T
  * sequences a token each (a fork's rows, or a batch's). rw i32 on the card: [base, step, W, then (col, off, len) a row];
  * row t's keys are `len` cache rows from `off` (its prefix; forks share one) and then its own steps, step i at cache row
@@ -177,6 +183,41 @@ int btb_b200_attn_decode(const void* q, const void* K, const void* V, void* out,
 int btb_b200_attn_decode_rows(const void* q, const void* K, const void* V, void* out, const void* rw, int T, int Hq,
                               int Hk, int D, long long hs, long long rs, float scale, void* part_m, void* part_l,
                               void* part_acc, void* cnt, int win, const void* sinks, int cap, void* stream);
+/* The rows layout's attention with the shared prefixes read once: the contract of btb_b200_attn_decode_rows (same q, cache,
+ * rw, window, sinks; a padding row's output is left as it was), but the rows whose prefix is the same (off, len) go over
+ * it together. A row agrees with btb_b200_attn_decode_rows to rounding, not to the bit: where its sums are cut depends on
+ * the lengths of all rows. D 64 or 128, Hq / Hk 1, 2, 4 or 8, T <= 32; q, K, V, out, workspace 16-byte aligned, hs and rs
+ * multiples of 8 with a row's kv heads inside its stride ((Hk - 1) hs + D <= rs) or each head's rows on their own (hs a
+ * multiple of rs, at least cap rows). workspace: btb_b200_attn_shared_workspace_bytes bytes (0 for a shape it refuses),
+ * no contents needed or kept; calls that may overlap need one each. */
+int btb_b200_attn_shared(const void* q, const void* K, const void* V, void* out, const void* rw, int T, int Hq, int Hk,
+                         int D, long long hs, long long rs, float scale, void* workspace, int win, const void* sinks,
+                         int cap, void* stream);
+size_t btb_b200_attn_shared_workspace_bytes(int T, int Hq, int Hk, int D); /* see btb_b200_attn_shared */
+/* btb_b200_attn_decode over a chain or tree pass of T <= 32 rows (no window) that also adds up what each cache row is
+ * given: totals f32, kv head g's at g * ts (ts >= cap), by LOGICAL row (before tbl). Rows j < n0 are added to,
+ * totals[g][j] += the softmax weights of row j over the pass's rows and the kv head's query heads; the pass's own rows
+ * n0 .. n0 + T - 1 are set to theirs; rows past them are left as they were. One order of summation: the same inputs give
+ * the same bits. Every parent is below its row. Refusals, shapes, alignment and workspace as btb_b200_attn_shared's; a
+ * pass that does not fit the cache writes nothing but the status word. */
+int btb_b200_attn_scored(const void* q, const void* K, const void* V, void* out, const void* n0p, const void* par, int T,
+                         int Hq, int Hk, int D, long long hs, long long rs, float scale, void* totals, long long ts,
+                         void* workspace, const void* tbl, const void* sinks, int cap, void* stream);
+size_t btb_b200_attn_scored_workspace_bytes(int T, int Hq, int Hk, int D, int cap); /* see btb_b200_attn_scored */
+/* Eviction by those totals (no counterpart in the reference). Of the n = *n0p rows that stand, each kv head of each layer
+ * keeps the `recent` last and, of the others, the keep - recent with the largest totals (equal totals: the lower row; a
+ * NaN ranks above all). The kept rows' keys, values and totals move, in order, to rows 0 .. keep - 1 of Kd, Vd, totals_d:
+ * the same cache (every pointer, stride and map equal: in place) or one that shares no row with it. With n <= keep every row is
+ * kept. K, V: layer a, kv head g, row r at a * ls + g * hs + r * rs (the destination's layers at ld); totals f32
+ * [layers, Hk, cap], totals_d [layers, Hk, cap_d]; idx i32 [layers, Hk, keep] gets the kept rows' old numbers (-1 past the
+ * count), n_out the count (may be n0p's own word: the rest of the cache then stands after it). Rows past the count are
+ * left as they were. tbl, tbl_d: logical row -> cache row of source and destination, or null. D a multiple of 8;
+ * 0 <= recent <= keep <= cap_d. workspace: btb_b200_kv_evict_workspace_bytes bytes, 16-byte aligned, no contents needed. */
+int btb_b200_kv_evict(const void* K, const void* V, const void* totals, const void* n0p, void* Kd, void* Vd,
+                      void* totals_d, void* n_out, void* idx, int layers, long long ls, long long ld, int Hk, int D,
+                      long long hs, long long rs, int cap, int cap_d, int keep, int recent, const void* tbl,
+                      const void* tbl_d, void* workspace, void* stream);
+size_t btb_b200_kv_evict_workspace_bytes(int layers, int Hk, int cap); /* see btb_b200_kv_evict */
 /* the decode step's row (T = 1) in one launch: btb_norm_rope_kv_d* (btb_kernels.cu:261-358) and btb_attn_flash_d*
  * (btb_attn_flash.cuh:372-675) back to back in the reference. Every block rotates its kv head's queries itself; the
  * block whose key group holds slot n0 makes the new key and value, writes them to the cache and uses them from shared
