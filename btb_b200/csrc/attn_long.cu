@@ -1,5 +1,9 @@
 // Attention over long caches for sm_100a. Two entry points: btb_b200_attn_shared, a pass in the rows layout whose rows
 // share prefixes, and btb_b200_attn_scored, a chain or tree pass that also adds up what each cache row is given.
+#include <cuda.h>
+
+#include <atomic>
+
 #include "common.cuh"
 #include "btb_b200_internal.h"
 #include "attn_core.cuh"
@@ -23,61 +27,605 @@ struct LongArgs {
     float* totals;       // [Hk, ts] what each logical row has been given, or null
     float* lse;          // [T, Hq] log2 of a row's denominator
     float* own;          // [T, Hq, 32] the scores of the pass's own rows in log2 units, -inf where not seen
+    float2* part_ml;     // a part's rows: maximum and sum ...
+    float* part_o;       // ... and output [., D], not yet divided
     float scale;
-    int T, Hq, Hk, win, cap;
+    int T, Hq, Hk, win, cap, ctas;
     long long hs, rs, ts;
 };
 
-// the logical keys of pass row t: [first, last], and the cache row of each
-struct Keys {
-    int first, last, n0;
-    RowSeq seq;
-    const int* anc;  // the pass's ancestors of t, root first (chain or tree pass)
-    const LongArgs& A;
-    __device__ __forceinline__ Keys(const LongArgs& a, int t, int n0_, const int* anc_, int len)
-        : n0(n0_), seq(a.rw, t, a.rw != nullptr), anc(anc_), A(a) {
-        last = a.rw != nullptr ? seq.position() : n0_ + len - 1;
-        first = a.win > 0 ? max(last + 1 - a.win, 0) : 0;
-    }
-    // -1, and the status word, for a row outside the cache: such a key is not read
-    __device__ __forceinline__ int row(int j) const {
-        int r;
-        if (A.rw != nullptr) {
-            r = seq.slot(j);
-        } else {
-            r = j < n0 ? j : n0 + anc[j - n0];
-            if (A.tbl != nullptr) r = A.tbl[r];
-        }
-        if (r >= 0 && r < A.cap) return r;
-        b2_fail(B2_ERR_DOMAIN);
-        return -1;
-    }
+// ---- the pass's work, from what stands on the card ------------------------------------------------------------------
+// Key tiles of 128 rows. Per kv head there is an item for each prefix that rows share - its queries are all of those rows' -
+// and, in the rows layout, one for each row's own steps as far as they fill whole tiles; the rest of a row's own (fewer
+// than 128 steps, or a chain or tree pass's at most 32 rows) is the joining kernel's. The tiles of all heads in one line
+// are cut evenly over the CTAs; a CTA's stretch of an item is a part, whose state (maximum, sum, output row) the joining
+// kernel folds with the others'. Part (CTA c, item i) keeps its rows at c * T G + the rows of all items before i, which no
+// two parts share.
+constexpr int KT = 128;        // keys a tile
+constexpr int CTAS_MAX = 160;  // CTAs of the tile kernel at most
+
+struct Plan {
+    int mask[32];                               // item of lane l's prefix: its rows (0: no item)
+    int p_start[32], p_count[32];               // ... its first key (cache row, or logical row of a chain or tree pass) and keys
+    int p_tiles[32], p_tile0[32], p_row0[32];   // ... tiles, tiles and partial rows before it (within a kv head)
+    int s_start[32], s_tiles[32], s_tile0[32], s_row0[32];  // the same of row l's own steps
+    int lead[32];                               // row t's prefix item, -1: padding or refused
+    int own[32], own_n[32];                     // its remaining steps: the first's cache row, how many
+    int W, tiles, rows, n0;                     // ... and the kv head's tiles and partial rows
 };
 
-constexpr int JW = 8;  // warps of a row's block
+__device__ __forceinline__ int warp_excl(int v, int lane, int& total) {
+    int x = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int u = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += u;
+    }
+    total = __shfl_sync(0xffffffffu, x, 31);
+    return x - v;
+}
 
-// One block a (row, kv head): its warps walk the keys 32 at a time with a running maximum and sum, a lane a key for the
-// scores and D / 32 dims for the output; the warps' states are folded at the end.
+// one warp fills `P`; `tell`: this block records a refused layout
+__device__ __forceinline__ void make_plan(const LongArgs& A, int G, Plan& P, bool tell) {
+    const int t = threadIdx.x & 31;
+    int mask = 0, start = 0, count = 0, s_start = 0, s_tiles = 0, lead = -1, own = 0, own_n = 0, W = 0, n0 = 0;
+    if (A.rw == nullptr) {
+        n0 = *A.n0p;
+        if (n0 < 0 || n0 > A.cap - A.T) {
+            if (tell && t == 0) b2_fail(B2_ERR_DOMAIN);
+        } else {
+            lead = t < A.T ? 0 : -1;
+            if (t == 0) mask = A.T == 32 ? -1 : (1 << A.T) - 1, count = n0;
+        }
+    } else {
+        const int base = A.rw[0], step = A.rw[1];
+        W = A.rw[2];
+        bool live = t < A.T;
+        const int col = live ? A.rw[3 + 3 * t] : 0, off = live ? A.rw[4 + 3 * t] : 0, len = live ? A.rw[5 + 3 * t] : -1;
+        live = live && len >= 0;
+        if (live) {
+            const long long lo = (long long)base + col, hi = lo + (long long)step * W;
+            if (step < 0 || W < 0 || off < 0 || len > A.cap || off > A.cap - len || lo < 0 || hi >= A.cap || step > A.cap) {
+                if (tell) b2_fail(B2_ERR_DOMAIN);
+                live = false;
+            }
+        }
+        const int first = A.win > 0 ? (int)max((long long)len + step + 1 - A.win, 0LL) : 0;
+        const unsigned alive = __ballot_sync(0xffffffffu, live);
+        const unsigned same = __match_any_sync(0xffffffffu, off) & __match_any_sync(0xffffffffu, len) & alive;
+        if (live) {
+            lead = __ffs(same) - 1;
+            if (lead == t) mask = same, start = off + first, count = max(0, len - first);
+            const int i0 = max(0, first - len), n = step + 1 - i0;
+            s_start = base + i0 * W + col;
+            s_tiles = n / KT;
+            own = s_start + s_tiles * KT * W, own_n = n - s_tiles * KT;
+        }
+    }
+    const int p_tiles = mask ? (count + KT - 1) / KT : 0;
+    int pt, st, pr, sr;
+    const int p_tile0 = warp_excl(p_tiles, t, pt), s_tile0 = warp_excl(s_tiles, t, st);
+    const int p_row0 = warp_excl(p_tiles ? __popc(mask) * G : 0, t, pr), s_row0 = warp_excl(s_tiles ? G : 0, t, sr);
+    P.mask[t] = mask, P.p_start[t] = start, P.p_count[t] = count, P.p_tiles[t] = p_tiles, P.p_tile0[t] = p_tile0, P.p_row0[t] = p_row0;
+    P.s_start[t] = s_start, P.s_tiles[t] = s_tiles, P.s_tile0[t] = pt + s_tile0, P.s_row0[t] = pr + s_row0;
+    P.lead[t] = lead, P.own[t] = own, P.own_n[t] = own_n;
+    if (t == 0) P.W = W, P.tiles = pt + st, P.rows = pr + sr, P.n0 = n0;
+    __syncwarp();
+}
+
+// where CTA c's stretch of `tiles` tiles begins; only as many of the `ctas` CTAs have one as there are tiles, so that no
+// stretch between two others is empty
+__device__ __forceinline__ long long first_tile(long long tiles, int c, int ctas) {
+    const long long n = min((long long)ctas, tiles);
+    return c >= n ? tiles : tiles * c / n;
+}
+
+// a CTA's stretch of one item
+struct Part {
+    int head, mask, start, stride, keys, tiles, rows;  // `keys`: of these tiles (the last may be partly filled)
+    long long row0;                                    // its first partial row
+    long long end;                                     // the first tile past it
+    bool prefix;
+};
+// the part that begins at tile `at` of a CTA whose stretch ends at `stop` (every lane of a warp asks alike)
+__device__ __forceinline__ Part part_at(const Plan& P, const LongArgs& A, int G, long long at, long long stop, int cta) {
+    const int lane = threadIdx.x & 31;
+    Part p;
+    p.head = (int)(at / P.tiles);
+    const int in = (int)(at - (long long)p.head * P.tiles);
+    const unsigned pp = __ballot_sync(0xffffffffu, in >= P.p_tile0[lane] && in < P.p_tile0[lane] + P.p_tiles[lane]);
+    const unsigned ss = __ballot_sync(0xffffffffu, in >= P.s_tile0[lane] && in < P.s_tile0[lane] + P.s_tiles[lane]);
+    p.prefix = pp != 0;
+    const int l = __ffs(p.prefix ? pp : ss) - 1;
+    const int tile0 = p.prefix ? P.p_tile0[l] : P.s_tile0[l], tiles = p.prefix ? P.p_tiles[l] : P.s_tiles[l];
+    const int skip = in - tile0;
+    p.tiles = (int)min((long long)(tiles - skip), stop - at);
+    p.mask = p.prefix ? P.mask[l] : 1 << l;
+    p.stride = p.prefix ? 1 : P.W;
+    p.start = (p.prefix ? P.p_start[l] : P.s_start[l]) + skip * KT * p.stride;
+    p.keys = min(p.tiles * KT, (p.prefix ? P.p_count[l] : tiles * KT) - skip * KT);
+    p.rows = __popc(p.mask) * G;
+    p.row0 = (long long)cta * A.T * G + (long long)p.head * P.rows + (p.prefix ? P.p_row0[l] : P.s_row0[l]);
+    p.end = at + p.tiles;
+    return p;
+}
+
+// ---- the tiles on the tensor cores -------------------------------------------------------------------------------------
+// S = Q K^T and O += P V with tcgen05.mma: up to 128 of an item's query rows (row-of-the-pass major, then the kv head's query
+// heads) are the MMA's M, so a shared key is read once for all of them. Two warpgroups turn scores into weights, a thread a
+// query row, on alternate key tiles with an output accumulator each (items of up to 128 rows; the two are folded at the
+// part's end) or on the two halves of an item's up to 256 rows. Scores, weights (over their scores) and outputs live in
+// tensor memory: S0 S1 O0 O1, 128 columns each.
+__device__ __forceinline__ uint64_t desc_sw128(uint32_t saddr, uint32_t lbo) {
+    return (uint64_t)((saddr & 0x3FFFFu) >> 4) | ((uint64_t)(lbo >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) |
+           ((uint64_t)2 << 61);
+}
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d), "l"(a),
+                 "l"(b), "r"(idesc), "r"(acc)
+                 : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d), "r"(a),
+                 "l"(b), "r"(idesc), "r"(acc)
+                 : "memory");
+}
+__device__ __forceinline__ void mma_commit(uint32_t bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void tm_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tm_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tm_ld32(uint32_t addr, uint32_t* r) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, "
+        "%24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+          "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]),
+          "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]),
+          "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(addr));
+}
+__device__ __forceinline__ void tm_ld16(uint32_t addr, uint32_t* r) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+          "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(addr));
+}
+__device__ __forceinline__ void tm_st16(uint32_t addr, const uint32_t* r) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(addr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+        "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        : "memory");
+}
+// the loads so far have arrived; the registers pass through, so that nothing reads them before
+__device__ __forceinline__ void tm_wait_ld(uint32_t (&r)[32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+        : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]),
+          "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]),
+          "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]),
+          "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
+        :
+        : "memory");
+}
+__device__ __forceinline__ void tm_wait_ld(uint32_t (&r)[16]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+        : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]),
+          "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+        :
+        : "memory");
+}
+__device__ __forceinline__ void tm_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tma_box(uint32_t dst, const CUtensorMap* tm, int x, int y, uint32_t bar) {
+    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+                 "l"(tm), "r"(x), "r"(y), "r"(bar)
+                 : "memory");
+}
+// four rows of 64 columns, wherever they lie
+__device__ __forceinline__ void tma_rows4(uint32_t dst, const CUtensorMap* tm, int x, const int* y, uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, %6}], "
+        "[%7];" ::"r"(dst),
+        "l"(tm), "r"(x), "r"(y[0]), "r"(y[1]), "r"(y[2]), "r"(y[3]), "r"(bar)
+        : "memory");
+}
+
+constexpr int TW = 10;          // warps: two warpgroups for the weights, the loads' warp, the MMAs' warp
+constexpr int STAGES_MAX = 6;   // stages of a ring
+
+struct alignas(8) TileSync {
+    uint64_t kfull[STAGES_MAX], kempty[STAGES_MAX], vfull[STAGES_MAX], vempty[STAGES_MAX];
+    uint64_t sfull[2];   // a warpgroup's scores are there
+    uint64_t pready[2];  // ... its weights are
+    uint64_t odone[2];   // ... its last product of a part is added
+    uint64_t qfull;      // the part's queries are in shared memory
+    uint64_t stats;      // the second warpgroup's maxima and sums are in shared memory
+    uint64_t next;       // both warpgroups are through with the part
+    uint64_t drain;      // every MMA has run
+    uint32_t tmem;
+    int fail;
+};
+
+struct TileArgs {
+    LongArgs a;
+    int row_mul, col_mul;  // a kv head's rows begin at head * row_mul, its columns at head * col_mul
+    int ks, vs;            // stages of the rings
+};
+
+// a warp's bounded wait that also ends once any other role has given up; its lanes get one answer
+__device__ __forceinline__ bool wait_or_fail(uint64_t* bar, uint32_t parity, TileSync& sy) {
+    const uint32_t b = smem_u32(bar);
+    bool ok = false;
+    uint32_t it = 0;
+    for (; it < B2_WAIT_LIMIT; ++it) {
+        if ((ok = mbar_try_wait(b, parity))) break;
+        if (*(volatile int*)&sy.fail) break;
+    }
+    if (it == B2_WAIT_LIMIT) *(volatile int*)&sy.fail = 1;
+    return __all_sync(0xffffffffu, ok);
+}
+
+template <int D>
+__global__ void __launch_bounds__(TW * 32, 1)
+    long_tiles(const __grid_constant__ CUtensorMap kbox, const __grid_constant__ CUtensorMap krows,
+               const __grid_constant__ CUtensorMap vbox, const __grid_constant__ CUtensorMap vrows, const TileArgs X) {
+    constexpr int TILE = KT * D * 2;    // bytes of a tile of keys, values or queries: D / 64 blocks of 128 rows x 128 bytes
+    constexpr int HALF = KT * 128;
+    const LongArgs& A = X.a;
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    __shared__ TileSync sy;
+    __shared__ Plan plan;
+    __shared__ float s_m[128], s_l[128];
+    uint8_t* smem = smem_raw;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int G = A.Hq / A.Hk, nq = A.T * G > 128 ? 2 : 1;
+    const uint32_t sq = smem_u32(smem), sk = sq + nq * TILE, sv = sk + X.ks * TILE;
+
+    pdl_launch_dependents();
+    pdl_wait();
+    if (warp == 0) make_plan(A, G, plan, blockIdx.x == 0);
+    if (threadIdx.x == 32) {
+        for (int s = 0; s < STAGES_MAX; ++s) {
+            mbar_init(smem_u32(&sy.kfull[s]), 1), mbar_init(smem_u32(&sy.kempty[s]), 1);
+            mbar_init(smem_u32(&sy.vfull[s]), 1), mbar_init(smem_u32(&sy.vempty[s]), 1);
+        }
+        for (int w = 0; w < 2; ++w)
+            mbar_init(smem_u32(&sy.sfull[w]), 1), mbar_init(smem_u32(&sy.pready[w]), 4), mbar_init(smem_u32(&sy.odone[w]), 1);
+        mbar_init(smem_u32(&sy.qfull), 8), mbar_init(smem_u32(&sy.stats), 4), mbar_init(smem_u32(&sy.next), 8);
+        mbar_init(smem_u32(&sy.drain), 1);
+        sy.fail = 0;
+        mbar_fence_init();
+    }
+    __syncthreads();
+    const long long all = (long long)plan.tiles * A.Hk;
+    const long long begin = first_tile(all, blockIdx.x, gridDim.x), stop = first_tile(all, blockIdx.x + 1, gridDim.x);
+    if (begin >= stop) return;  // (no work for this CTA: nothing allocated yet)
+    if (sq & 1023) {  // (the tiles take all but 3 KB of what a block may have: there is no room to align them here)
+        if (threadIdx.x == 0) b2_fail(B2_ERR_CUDA);
+        return;
+    }
+    if (warp == 9) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sy.tmem)), "r"(512u) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tm_before();
+    __syncthreads();
+    tm_after();
+    const uint32_t tmem = sy.tmem;
+
+    if (warp < 8) {
+        // ---- the weights: thread = query row of the tile ------------------------------------------------------------------
+        const int wg = warp >> 2, row = threadIdx.x & 127;
+        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+        const uint32_t ts = tmem + lanes + wg * 128, to = tmem + lanes + 256 + wg * 128;
+        const float scale2 = fabsf(__fmul_rn(A.scale, LOG2E));  // (a negative scale's sign is the queries')
+        uint32_t sph = 0, oph = 0, stph = 0, nph = 0;
+        bool ok = true;
+        for (long long at = begin; at < stop && ok;) {
+            const Part p = part_at(plan, A, G, at, stop, blockIdx.x);
+            at = p.end;
+            const bool two = p.rows > 128;
+            {   // the part's queries into shared memory as the MMA reads them: 16-byte piece c of row r at c ^ (r & 7)
+                const uint32_t flip = A.scale < 0.f ? 0x80008000u : 0u;
+                for (int rt = 0; rt < (two ? 2 : 1); ++rt) {
+                    const int r = rt * 128 + row;
+                    const int t = r < p.rows ? (int)__fns(p.mask, 0, r / G + 1) : 0;
+                    const uint4* src = reinterpret_cast<const uint4*>(A.q + ((size_t)t * A.Hq + p.head * G + r % G) * D) + wg * (D / 16);
+#pragma unroll
+                    for (int c = 0; c < D / 16; ++c) {
+                        uint4 v = r < p.rows ? src[c] : make_uint4(0u, 0u, 0u, 0u);
+                        v.x ^= flip, v.y ^= flip, v.z ^= flip, v.w ^= flip;
+                        const int piece = wg * (D / 16) + c;
+                        *reinterpret_cast<uint4*>(smem + rt * TILE + (piece >> 3) * HALF + row * 128 + (((piece & 7) ^ (row & 7)) << 4)) = v;
+                    }
+                }
+                fence_proxy_async();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(smem_u32(&sy.qfull));
+            }
+            const int mine = two ? p.tiles : (p.tiles + 1 - wg) >> 1;  // this warpgroup's tiles
+            const int valid = two ? p.rows - wg * 128 : p.rows;        // ... and query rows
+            const bool idle = (warp & 3) * 32 >= valid;
+            float m = NEG_INF, l = 0.f;
+            for (int i = 0; i < mine; ++i) {
+                if (!(ok = wait_or_fail(&sy.sfull[wg], sph, sy))) break;
+                sph ^= 1;
+                tm_after();
+                if (!idle) {
+                    const int left = p.keys - (two ? i : 2 * i + wg) * KT;  // keys from this tile's first on
+                    // (the scores are read twice, for the maximum and for the weights: held over, they would spill)
+                    uint32_t s[2][32];
+                    float mx[4] = {NEG_INF, NEG_INF, NEG_INF, NEG_INF};
+                    tm_ld32(ts, s[0]);
+#pragma unroll
+                    for (int c0 = 0; c0 < KT; c0 += 32) {
+                        uint32_t(&v)[32] = s[(c0 >> 5) & 1];
+                        tm_wait_ld(v);
+                        tm_ld32(ts + (c0 + 32 < KT ? c0 + 32 : 0), s[((c0 >> 5) & 1) ^ 1]);  // (last: the first again)
+                        if (left < c0 + 32) {
+#pragma unroll
+                            for (int c = 0; c < 32; ++c) v[c] = c0 + c < left ? v[c] : 0xff800000u;
+                        }
+#pragma unroll
+                        for (int c = 0; c < 32; ++c) mx[c & 3] = fmaxf(mx[c & 3], __uint_as_float(v[c]));
+                    }
+                    const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale2;
+                    // The weights are taken relative to a reference that follows the maximum only when that has risen by more
+                    // than 8 (a factor of 256, which sums and bf16 weights hold without loss): most tiles leave the output alone.
+                    const float ref = i == 0 ? top : (top > m + 8.f ? top : m);
+                    if (i > 0 && __any_sync(0xffffffffu, ref != m)) {
+                        const float f = m == NEG_INF ? 0.f : ex2(m - ref);
+                        l *= f;
+#pragma unroll 1
+                        for (int c = 0; c < D; c += 16) {
+                            uint32_t o[16];
+                            tm_ld16(to + c, o);
+                            tm_wait_ld(o);
+#pragma unroll
+                            for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
+                            tm_st16(to + c, o);
+                        }
+                    }
+                    m = ref;
+                    const float sub = m == NEG_INF ? 0.f : m;
+                    float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int c0 = 0; c0 < KT; c0 += 32) {
+                        uint32_t(&v)[32] = s[(c0 >> 5) & 1];
+                        uint32_t w[16];
+                        tm_wait_ld(v);
+                        if (c0 + 32 < KT) tm_ld32(ts + c0 + 32, s[((c0 >> 5) & 1) ^ 1]);
+                        if (left < c0 + 32) {
+#pragma unroll
+                            for (int c = 0; c < 32; ++c) v[c] = c0 + c < left ? v[c] : 0xff800000u;
+                        }
+#pragma unroll
+                        for (int c = 0; c < 16; ++c) {
+                            const float a = ex2(fmaf(__uint_as_float(v[2 * c]), scale2, -sub));
+                            const float b = ex2(fmaf(__uint_as_float(v[2 * c + 1]), scale2, -sub));
+                            sum[(2 * c) & 3] += a, sum[(2 * c + 1) & 3] += b;
+                            asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w[c]) : "f"(b), "f"(a));
+                        }
+                        tm_st16(ts + c0 / 2, w);
+                    }
+                    l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                    tm_wait_st();
+                }
+                tm_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(smem_u32(&sy.pready[wg]));
+            }
+            // ---- the part's state ----------------------------------------------------------------------------------------
+            if (ok && mine > 0) {
+                ok = wait_or_fail(&sy.odone[wg], oph, sy);
+                oph ^= 1;
+                tm_after();
+            }
+            if (!two && wg == 1) {
+                s_m[row] = mine > 0 ? m : NEG_INF, s_l[row] = l;
+                tm_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(smem_u32(&sy.stats));
+            }
+            if (!two && wg == 0 && ok) {
+                ok = wait_or_fail(&sy.stats, stph, sy);
+                tm_after();
+            }
+            if (!two) stph ^= 1;
+            if (ok && !idle && (two || wg == 0)) {
+                const int r = wg * 128 + row;  // (two: the warpgroup's half; else the first's)
+                const bool other = !two && p.tiles > 1;
+                float f0 = 1.f, f1 = 0.f, M = m, L = l;
+                if (other) {
+                    fold_ml(M, L, s_m[row], s_l[row], f0, f1);
+                }
+                const size_t at_row = (size_t)(p.row0 + r);
+#pragma unroll 1
+                for (int c = 0; c < D; c += 32) {
+                    uint32_t o[32], o2[32];
+                    tm_ld32(to + c, o);
+                    if (other) {
+                        tm_ld32(to + 128 + c, o2);
+                        tm_wait_ld(o2);
+                    }
+                    tm_wait_ld(o);
+                    if (row < valid) {
+#pragma unroll
+                        for (int k = 0; k < 32; k += 4) {
+                            float4 v = make_float4(__uint_as_float(o[k]), __uint_as_float(o[k + 1]), __uint_as_float(o[k + 2]),
+                                                   __uint_as_float(o[k + 3]));
+                            if (other) {
+                                v.x = fold_e(v.x, __uint_as_float(o2[k]), f0, f1), v.y = fold_e(v.y, __uint_as_float(o2[k + 1]), f0, f1);
+                                v.z = fold_e(v.z, __uint_as_float(o2[k + 2]), f0, f1), v.w = fold_e(v.w, __uint_as_float(o2[k + 3]), f0, f1);
+                            }
+                            *reinterpret_cast<float4*>(A.part_o + at_row * D + c + k) = v;
+                        }
+                    }
+                }
+                if (row < valid) A.part_ml[at_row] = make_float2(M, L);
+            }
+            tm_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&sy.next));
+            if (ok) ok = wait_or_fail(&sy.next, nph, sy);
+            nph ^= 1;
+            tm_after();
+        }
+    } else if (warp == 8) {
+        // ---- the loads --------------------------------------------------------------------------------------------------------
+        int ks = 0, vs = 0;
+        uint32_t kph = 0, vph = 0;
+        long long kn = 0, vn = 0;  // tiles begun
+        bool ok = true;
+        for (long long at = begin; at < stop && ok;) {
+            const Part p = part_at(plan, A, G, at, stop, blockIdx.x);
+            at = p.end;
+            const int x = p.head * X.col_mul, y0 = p.head * X.row_mul;
+            const bool mapped = p.prefix && A.tbl != nullptr;
+            for (int i = 0; i < p.tiles && ok; ++i) {
+                const int keys = min(KT, p.keys - i * KT);
+                const bool box = keys == KT && p.stride == 1 && !mapped;
+                int y[4];
+                if (box) {
+                    y[0] = y0 + p.start + i * KT;
+                } else {
+                    // rows 4 lane .. 4 lane + 3 of the tile; past its keys the last one again (its weight there is 0: the
+                    // values multiplied by it must be ones that the rows see)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const int j = p.start + (i * KT + min(lane * 4 + k, keys - 1)) * p.stride;
+                        int r = mapped ? A.tbl[j] : j;
+                        if (r < 0 || r >= A.cap) {
+                            b2_fail(B2_ERR_DOMAIN);
+                            r = 0;
+                        }
+                        y[k] = y0 + r;
+                    }
+                }
+                for (int kv = 0; kv < 2 && ok; ++kv) {
+                    uint64_t* full = kv == 0 ? &sy.kfull[ks] : &sy.vfull[vs];
+                    uint64_t* empty = kv == 0 ? &sy.kempty[ks] : &sy.vempty[vs];
+                    const bool used = kv == 0 ? kn >= X.ks : vn >= X.vs;
+                    if (used && !(ok = wait_or_fail(empty, (kv == 0 ? kph : vph) ^ 1, sy))) break;
+                    const uint32_t bar = smem_u32(full), dst = kv == 0 ? sk + ks * TILE : sv + vs * TILE;
+                    if (lane == 0) mbar_expect_tx(bar, TILE);
+                    __syncwarp();
+                    if (box) {
+                        if (lane == 0)
+                            for (int c = 0; c < D / 64; ++c) tma_box(dst + c * HALF, kv == 0 ? &kbox : &vbox, x + c * 64, y[0], bar);
+                    } else {
+                        for (int c = 0; c < D / 64; ++c) tma_rows4(dst + c * HALF + lane * 512, kv == 0 ? &krows : &vrows, x + c * 64, y, bar);
+                    }
+                    if (kv == 0) {
+                        ++kn;
+                        if (++ks == X.ks) ks = 0, kph ^= 1;
+                    } else {
+                        ++vn;
+                        if (++vs == X.vs) vs = 0, vph ^= 1;
+                    }
+                }
+            }
+        }
+        // its copies have landed before the CTA ends (they have, unless some role gave up)
+        for (int s = 0; s < X.ks; ++s) {
+            const long long uses = kn / X.ks + (s < kn % X.ks ? 1 : 0);
+            if (uses > 0) (void)mbar_wait_bounded(smem_u32(&sy.kfull[s]), (uint32_t)(uses - 1) & 1);
+        }
+        for (int s = 0; s < X.vs; ++s) {
+            const long long uses = vn / X.vs + (s < vn % X.vs ? 1 : 0);
+            if (uses > 0) (void)mbar_wait_bounded(smem_u32(&sy.vfull[s]), (uint32_t)(uses - 1) & 1);
+        }
+    } else {
+        // ---- the MMAs -----------------------------------------------------------------------------------------------------------
+        // D f32, A and B bf16; S: both K-major, N = 128 keys; O: the values' dims are B's N and lie contiguous, N = D
+        constexpr uint32_t base_desc = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(128 >> 4) << 24);
+        constexpr uint32_t desc_s = base_desc | ((uint32_t)(KT >> 3) << 17), desc_o = base_desc | (1u << 16) | ((uint32_t)(D >> 3) << 17);
+        int ks = 0, vs = 0;
+        uint32_t kph = 0, vph = 0, pph[2] = {0, 0}, qph = 0;
+        bool ok = true;
+        for (long long at = begin; at < stop && ok;) {
+            const Part p = part_at(plan, A, G, at, stop, blockIdx.x);
+            at = p.end;
+            const int nrt = p.rows > 128 ? 2 : 1, jobs = p.tiles * nrt;
+            if (!(ok = wait_or_fail(&sy.qfull, qph, sy))) break;
+            qph ^= 1;
+            tm_after();
+            for (int j = -2; j < jobs && ok; ++j) {
+                if (j >= 0) {  // the output's share of job j
+                    const int w = j & 1;
+                    if ((nrt == 1 || w == 0) && !(ok = wait_or_fail(&sy.vfull[vs], vph, sy))) break;
+                    if (!(ok = wait_or_fail(&sy.pready[w], pph[w], sy))) break;
+                    pph[w] ^= 1;
+                    tm_after();
+                    if (lane == 0) {
+                        const uint64_t b = desc_sw128(sv + vs * TILE, HALF);
+#pragma unroll
+                        for (int k = 0; k < KT / 16; ++k)
+                            mma_ts(tmem + 256 + w * 128, tmem + w * 128 + k * 8, b + k * (2048 >> 4), desc_o, j >= 2 || k > 0);
+                        if (nrt == 1 || w == 1) mma_commit(smem_u32(&sy.vempty[vs]));
+                        if (j >= jobs - 2) mma_commit(smem_u32(&sy.odone[w]));
+                    }
+                    if (nrt == 1 || w == 1)
+                        if (++vs == X.vs) vs = 0, vph ^= 1;
+                }
+                const int n = j + 2;
+                if (n < jobs) {  // the scores of job j + 2, over job j's
+                    const int w = n & 1;
+                    if ((nrt == 1 || w == 0) && !(ok = wait_or_fail(&sy.kfull[ks], kph, sy))) break;
+                    tm_after();
+                    if (lane == 0) {
+                        const uint64_t qa = desc_sw128(sq + (nrt == 2 ? w * TILE : 0), 0), kb = desc_sw128(sk + ks * TILE, 0);
+#pragma unroll
+                        for (int k = 0; k < D / 16; ++k) {
+                            const uint64_t o = (uint64_t)(((k >> 2) * HALF + (k & 3) * 32) >> 4);
+                            mma_ss(tmem + w * 128, qa + o, kb + o, desc_s, k > 0);
+                        }
+                        mma_commit(smem_u32(&sy.sfull[w]));
+                        if (nrt == 1 || w == 1) mma_commit(smem_u32(&sy.kempty[ks]));
+                    }
+                    if (nrt == 1 || w == 1)
+                        if (++ks == X.ks) ks = 0, kph ^= 1;
+                }
+                __syncwarp();
+            }
+        }
+        if (lane == 0) {
+            mma_commit(smem_u32(&sy.drain));
+            (void)mbar_wait_bounded(smem_u32(&sy.drain), 0);
+        }
+        __syncwarp();
+    }
+    tm_before();
+    __syncthreads();
+    if (threadIdx.x == 0 && sy.fail) b2_fail(B2_ERR_TIMEOUT);
+    if (warp == 9) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+}
+
+// ---- a row's parts joined ------------------------------------------------------------------------------------------------
+constexpr int JW = KT / 32;                    // warps of a row's block
+constexpr int PARTS_MAX = 2 * (CTAS_MAX + 1);  // parts of a row's prefix and own steps
+
+// One block a (row, kv head): its warps take the row's remaining own keys 32 at a time (a lane a key for the scores, D / 32
+// dims for the output; keys outside are never touched), then their states, the parts' and the sink are folded.
 template <int D, int G>
-__global__ void __launch_bounds__(JW * 32) long_rows(const LongArgs A) {
+__global__ void __launch_bounds__(JW * 32) long_join(const LongArgs A) {
     constexpr int E = D / 32;
+    __shared__ Plan plan;
     __shared__ __align__(16) uint32_t qs[G][D / 2];
     __shared__ float ps[JW][G][32];
     __shared__ float wm[JW][G], wl[JW][G];
     __shared__ float wo[JW][G][D];
+    __shared__ float fac[G][PARTS_MAX];
+    __shared__ float top[G], den[G];
     __shared__ int anc[TMAX];
     __shared__ int s_len;
     pdl_launch_dependents();
     pdl_wait();
     const int t = blockIdx.x, g = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int n0 = A.rw != nullptr ? 0 : *A.n0p;
-    if (A.rw != nullptr) {
-        if (A.rw[5 + 3 * t] < 0) return;  // padding
-    } else if (n0 < 0 || n0 > A.cap - A.T) {
-        if (threadIdx.x == 0) b2_fail(B2_ERR_DOMAIN);
-        return;
-    }
-    if (threadIdx.x == 0) {
+    if (warp == 0) make_plan(A, G, plan, false);
+    if (threadIdx.x == 32) {
         int len = 0;
         if (A.rw == nullptr) {
             for (int p = t; p >= 0 && p < A.T && len < TMAX; p = A.par[p]) ++len;
@@ -93,7 +641,9 @@ __global__ void __launch_bounds__(JW * 32) long_rows(const LongArgs A) {
     if (A.own != nullptr)
         for (int i = threadIdx.x; i < G * 32; i += JW * 32) A.own[((size_t)t * A.Hq + g * G) * 32 + i] = NEG_INF;
     __syncthreads();
-    const Keys keys(A, t, n0, anc, s_len);
+    const int lead = plan.lead[t];
+    if (lead < 0) return;  // padding, or refused
+    const int n = A.rw != nullptr ? plan.own_n[t] : s_len;
     const float scale2 = __fmul_rn(A.scale, LOG2E);
     const bf16* Kg = A.K + (size_t)g * A.hs;
     const bf16* Vg = A.V + (size_t)g * A.hs;
@@ -104,15 +654,27 @@ __global__ void __launch_bounds__(JW * 32) long_rows(const LongArgs A) {
 #pragma unroll
         for (int e = 0; e < E; ++e) o[hh][e] = 0.f;
     }
-    for (int j0 = keys.first + warp * 32; j0 <= keys.last; j0 += JW * 32) {
-        const int j = j0 + lane;
-        const int row = j <= keys.last ? keys.row(j) : -1;
+    const int i = warp * 32 + lane;  // (at most 127 keys: a warp's one stretch)
+    if (warp * 32 < n) {
+        int row = -1;
+        if (i < n) {
+            if (A.rw != nullptr) {
+                row = plan.own[t] + i * plan.W;
+            } else {
+                row = plan.n0 + anc[i];
+                if (A.tbl != nullptr) row = A.tbl[row];
+                if (row < 0 || row >= A.cap) {
+                    b2_fail(B2_ERR_DOMAIN);
+                    row = -1;
+                }
+            }
+        }
         float s[G];
 #pragma unroll
         for (int hh = 0; hh < G; ++hh) s[hh] = 0.f;
         if (row >= 0) {
             const uint4* kr = reinterpret_cast<const uint4*>(Kg + (size_t)row * A.rs);
-#pragma unroll 4
+#pragma unroll 8
             for (int c = 0; c < D / 8; ++c) {
                 const uint4 kv = __ldg(kr + c);
 #pragma unroll
@@ -125,32 +687,26 @@ __global__ void __launch_bounds__(JW * 32) long_rows(const LongArgs A) {
 #pragma unroll
         for (int hh = 0; hh < G; ++hh) {
             s[hh] = row >= 0 ? __fmul_rn(s[hh], scale2) : NEG_INF;
-            if (A.own != nullptr && j >= n0 && j <= keys.last)
-                A.own[((size_t)t * A.Hq + g * G + hh) * 32 + anc[j - n0]] = s[hh];
+            if (A.own != nullptr && i < n) A.own[((size_t)t * A.Hq + g * G + hh) * 32 + anc[i]] = s[hh];
             float mx = s[hh];
 #pragma unroll
             for (int k = 16; k > 0; k >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, k));
-            const float mn = fmaxf(m[hh], mx);
-            const float c = m[hh] == NEG_INF ? 0.f : ex2(m[hh] - mn);
-            const float p = s[hh] == NEG_INF ? 0.f : ex2(s[hh] - mn);
-            l[hh] = l[hh] * c + warp_sum(p);
-            m[hh] = mn;
+            const float p = s[hh] == NEG_INF ? 0.f : ex2(s[hh] - mx);
+            l[hh] = warp_sum(p);
+            m[hh] = mx;
             ps[warp][hh][lane] = p;
-#pragma unroll
-            for (int e = 0; e < E; ++e) o[hh][e] *= c;
         }
         __syncwarp();
-        for (int i = 0; i < 32; ++i) {
-            const int r = __shfl_sync(0xffffffffu, row, i);
+        for (int k = 0; k < 32; ++k) {
+            const int r = __shfl_sync(0xffffffffu, row, k);
             if (r < 0) continue;
             __align__(8) bf16 v[E];
             ld_run<E, false>(Vg + (size_t)r * A.rs + lane * E, v);
 #pragma unroll
             for (int hh = 0; hh < G; ++hh)
 #pragma unroll
-                for (int e = 0; e < E; ++e) o[hh][e] = fmaf(ps[warp][hh][i], bf2f(v[e]), o[hh][e]);
+                for (int e = 0; e < E; ++e) o[hh][e] = fmaf(ps[warp][hh][k], bf2f(v[e]), o[hh][e]);
         }
-        __syncwarp();
     }
 #pragma unroll
     for (int hh = 0; hh < G; ++hh) {
@@ -158,20 +714,77 @@ __global__ void __launch_bounds__(JW * 32) long_rows(const LongArgs A) {
 #pragma unroll
         for (int e = 0; e < E; ++e) wo[warp][hh][lane * E + e] = o[hh][e];
     }
+    // the parts: those of the prefix's item, then those of the row's own steps; part k of an item is the k-th CTA's that
+    // holds tiles of it
+    const long long all = (long long)plan.tiles * A.Hk, head0 = (long long)g * plan.tiles, row_g = (long long)g * plan.rows;
+    int np = 0, ns = 0, pc = 0, sc = 0;
+    auto cta_of = [&](long long tile) {  // the CTA whose stretch holds `tile`
+        int c = (int)(tile * min((long long)A.ctas, all) / all);
+        while (first_tile(all, c, A.ctas) > tile) --c;
+        while (first_tile(all, c + 1, A.ctas) <= tile) ++c;
+        return c;
+    };
+    if (plan.p_tiles[lead] > 0) {
+        pc = cta_of(head0 + plan.p_tile0[lead]);
+        np = cta_of(head0 + plan.p_tile0[lead] + plan.p_tiles[lead] - 1) - pc + 1;
+    }
+    if (plan.s_tiles[t] > 0) {
+        sc = cta_of(head0 + plan.s_tile0[t]);
+        ns = cta_of(head0 + plan.s_tile0[t] + plan.s_tiles[t] - 1) - sc + 1;
+    }
+    const int below = __popc(plan.mask[lead] & ((1u << t) - 1u));  // the row's place among its prefix's
+    auto part_row = [&](int k) {
+        return k < np ? (long long)(pc + k) * A.T * G + row_g + plan.p_row0[lead] + below * G
+                      : (long long)(sc + k - np) * A.T * G + row_g + plan.s_row0[t];
+    };
     __syncthreads();
-    for (int i = threadIdx.x; i < G * D; i += JW * 32) {
-        const int hh = i / D, d = i - hh * D, head = g * G + hh;
-        float M = NEG_INF, L = 0.f, O = 0.f, cO, co;
-        for (int w = 0; w < JW; ++w) {
-            fold_ml(M, L, wm[w][hh], wl[w][hh], cO, co);
-            O = fold_e(O, wo[w][hh][d], cO, co);
+    for (int hh = warp; hh < G; hh += JW) {  // a warp a head: the largest maximum, each state's factor, the sum
+        float M = lane < JW ? wm[lane][hh] : NEG_INF;
+        for (int k = lane; k < np + ns; k += 32) M = fmaxf(M, A.part_ml[part_row(k) + hh].x);
+        const float sink = A.sinks != nullptr ? __fmul_rn(A.sinks[g * G + hh], LOG2E) : NEG_INF;
+        M = fmaxf(M, sink);
+#pragma unroll
+        for (int k = 16; k > 0; k >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, k));
+        const float sub = M == NEG_INF ? 0.f : M;
+        float L = 0.f;
+        if (lane < JW) {
+            const float f = wm[lane][hh] == NEG_INF ? 0.f : ex2(wm[lane][hh] - sub);
+            L += f * wl[lane][hh];
+            wm[lane][hh] = f;
         }
-        if (A.sinks != nullptr) {
-            fold_ml(M, L, __fmul_rn(A.sinks[head], LOG2E), 1.f, cO, co);
-            O = __fmul_rn(O, cO);
+        for (int k = lane; k < np + ns; k += 32) {
+            const float2 ml = A.part_ml[part_row(k) + hh];
+            const float f = ml.x == NEG_INF ? 0.f : ex2(ml.x - sub);
+            L += f * ml.y;
+            fac[hh][k] = f;
         }
-        A.out[((size_t)t * A.Hq + head) * D + d] = f2bf(__fdiv_rn(O, L));
-        if (d == 0 && A.lse != nullptr) A.lse[(size_t)t * A.Hq + head] = M + log2f(L);
+        L = warp_sum(L);
+        if (lane == 0) {
+            if (A.sinks != nullptr) L += ex2(sink - sub);
+            top[hh] = M, den[hh] = L;
+        }
+    }
+    __syncthreads();
+    for (int i4 = threadIdx.x; i4 < G * D / 4; i4 += JW * 32) {
+        const int hh = i4 / (D / 4), d = (i4 - hh * (D / 4)) * 4, head = g * G + hh;
+        float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int w = 0; w * 32 < n; ++w) {
+            const float f = wm[w][hh];
+            const float4 v = *reinterpret_cast<const float4*>(&wo[w][hh][d]);
+            O.x = fmaf(f, v.x, O.x), O.y = fmaf(f, v.y, O.y), O.z = fmaf(f, v.z, O.z), O.w = fmaf(f, v.w, O.w);
+        }
+#pragma unroll 4
+        for (int k = 0; k < np + ns; ++k) {
+            const float f = fac[hh][k];
+            const float4 v = *reinterpret_cast<const float4*>(A.part_o + (size_t)(part_row(k) + hh) * D + d);
+            O.x = fmaf(f, v.x, O.x), O.y = fmaf(f, v.y, O.y), O.z = fmaf(f, v.z, O.z), O.w = fmaf(f, v.w, O.w);
+        }
+        const float L = den[hh];
+        __nv_bfloat162 a, b;
+        a.x = f2bf(__fdiv_rn(O.x, L)), a.y = f2bf(__fdiv_rn(O.y, L)), b.x = f2bf(__fdiv_rn(O.z, L)), b.y = f2bf(__fdiv_rn(O.w, L));
+        __nv_bfloat162* out = reinterpret_cast<__nv_bfloat162*>(A.out + ((size_t)t * A.Hq + head) * D + d);
+        out[0] = a, out[1] = b;
+        if (d == 0 && A.lse != nullptr) A.lse[(size_t)t * A.Hq + head] = top[hh] + log2f(L);
     }
 }
 
@@ -224,9 +837,66 @@ __global__ void __launch_bounds__(WK) long_weights(const LongArgs A) {
     tot[j] += a;
 }
 
+typedef CUresult (*EncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                             const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion,
+                             CUtensorMapFloatOOBfill);
+// a cache of `rows` rows of `cols` elements, `stride` elements apart, in boxes of box_rows x 64 under the 128-byte swizzle
+int make_map(CUtensorMap* tm, const void* base, long long rows, long long cols, long long stride, int box_rows) {
+    static std::atomic<EncodeFn> known{nullptr};
+    EncodeFn fn = known.load(std::memory_order_acquire);
+    if (fn == nullptr) {
+        cudaDriverEntryPointQueryResult q;
+        void* p = nullptr;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess || p == nullptr) {
+            (void)cudaGetLastError();
+            return B2_ERR_CUDA;
+        }
+        fn = reinterpret_cast<EncodeFn>(p);
+        known.store(fn, std::memory_order_release);
+    }
+    const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)stride * 2};
+    const cuuint32_t box[2] = {64, (cuuint32_t)box_rows}, es[2] = {1, 1};
+    return fn(tm, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(base), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS
+               ? B2_OK
+               : B2_ERR_DOMAIN;
+}
+
+int long_ctas() { return min(b2_sm_count(), CTAS_MAX); }
+// partial rows at most: every CTA's stretch moves on by one item's rows, every kv head by its items'
+size_t part_rows(int T, int Hq) { return (size_t)long_ctas() * T * Hq + (size_t)2 * T * Hq; }
+
+template <int D>
+int launch_tiles(const LongArgs& a, cudaStream_t s) {
+    TileArgs x{};
+    x.a = a;
+    const int G = a.Hq / a.Hk;
+    const bool by_row = a.Hk == 1 || (a.Hk - 1) * a.hs + D <= a.rs;  // kv heads inside a cache row
+    const long long rows = by_row ? a.cap : (a.Hk - 1) * (a.hs / a.rs) + a.cap, cols = by_row ? (a.Hk - 1) * (a.Hk > 1 ? a.hs : 0) + D : D;
+    if (rows > 0x7fffffffLL || cols > 0x7fffffffLL) return B2_ERR_DOMAIN;
+    x.row_mul = by_row ? 0 : (int)(a.hs / a.rs), x.col_mul = by_row && a.Hk > 1 ? (int)a.hs : 0;
+    CUtensorMap tm[4];
+    for (int k = 0; k < 4; ++k)
+        if (const int rc = make_map(&tm[k], k < 2 ? a.K : a.V, rows, cols, a.rs, k & 1 ? 1 : KT)) return rc;
+    const int tile = KT * D * 2, nq = a.T * G > 128 ? 2 : 1, stages = (224 * 1024 - nq * tile) / tile;
+    x.vs = min(stages / 2, STAGES_MAX), x.ks = min(stages - x.vs, STAGES_MAX);
+    const size_t smem = (size_t)(nq + x.ks + x.vs) * tile;
+    auto kern = long_tiles<D>;
+    static bool allowed[64];
+    if (const int rc = b2_allow_smem(reinterpret_cast<const void*>(kern), allowed)) return rc;
+    cudaLaunchConfig_t cfg;
+    memset(&cfg, 0, sizeof cfg);
+    cfg.gridDim = dim3(a.ctas), cfg.blockDim = dim3(TW * 32), cfg.dynamicSmemBytes = smem, cfg.stream = s;
+    if (cudaLaunchKernelEx(&cfg, kern, tm[0], tm[1], tm[2], tm[3], x) != cudaSuccess) {
+        (void)cudaGetLastError();
+        return B2_ERR_CUDA;
+    }
+    return B2_OK;
+}
 template <int D, int G>
 int launch_long(const LongArgs& a, cudaStream_t s) {
-    if (const int rc = b2_launch(reinterpret_cast<const void*>(long_rows<D, G>), dim3(a.T, a.Hk), dim3(JW * 32), 0, s, a)) return rc;
+    if (const int rc = launch_tiles<D>(a, s)) return rc;
+    if (const int rc = b2_launch(reinterpret_cast<const void*>(long_join<D, G>), dim3(a.T, a.Hk), dim3(JW * 32), 0, s, a)) return rc;
     if (a.totals == nullptr) return B2_OK;
     auto kern = long_weights<D, G>;
     static bool allowed[64];
@@ -263,7 +933,7 @@ int check_cache(const void* q, const void* K, const void* V, const void* out, in
 }  // namespace
 
 extern "C" size_t btb_b200_attn_shared_workspace_bytes(int T, int Hq, int Hk, int D) {
-    return shape_ok(T, Hq, Hk, D) ? 16 : 0;
+    return shape_ok(T, Hq, Hk, D) ? part_rows(T, Hq) * (D * 4 + 8) : 0;
 }
 
 extern "C" int btb_b200_attn_shared(const void* q, const void* K, const void* V, void* out, const void* rw, int T, int Hq,
@@ -274,13 +944,14 @@ extern "C" int btb_b200_attn_shared(const void* q, const void* K, const void* V,
     LongArgs a{};
     a.q = static_cast<const bf16*>(q), a.K = static_cast<const bf16*>(K), a.V = static_cast<const bf16*>(V);
     a.out = static_cast<bf16*>(out), a.rw = static_cast<const int*>(rw), a.sinks = static_cast<const float*>(sinks);
-    a.scale = scale, a.T = T, a.Hq = Hq, a.Hk = Hk, a.win = win, a.cap = cap, a.hs = hs, a.rs = rs;
+    a.scale = scale, a.T = T, a.Hq = Hq, a.Hk = Hk, a.win = win, a.cap = cap, a.ctas = long_ctas(), a.hs = hs, a.rs = rs;
+    a.part_o = static_cast<float*>(workspace), a.part_ml = reinterpret_cast<float2*>(a.part_o + part_rows(T, Hq) * D);
     return D == 64 ? launch_long_g<64>(a, static_cast<cudaStream_t>(stream)) : launch_long_g<128>(a, static_cast<cudaStream_t>(stream));
 }
 
 extern "C" size_t btb_b200_attn_scored_workspace_bytes(int T, int Hq, int Hk, int D, int cap) {
     if (!shape_ok(T, Hq, Hk, D) || cap <= 0) return 0;
-    return (size_t)T * Hq * 33 * 4;
+    return part_rows(T, Hq) * (D * 4 + 8) + (size_t)T * Hq * 33 * 4;
 }
 
 extern "C" int btb_b200_attn_scored(const void* q, const void* K, const void* V, void* out, const void* n0p, const void* par,
@@ -294,7 +965,8 @@ extern "C" int btb_b200_attn_scored(const void* q, const void* K, const void* V,
     a.out = static_cast<bf16*>(out), a.n0p = static_cast<const int*>(n0p), a.par = static_cast<const int*>(par);
     a.tbl = static_cast<const int*>(tbl), a.sinks = static_cast<const float*>(sinks);
     a.totals = static_cast<float*>(totals), a.ts = ts;
-    a.lse = static_cast<float*>(workspace), a.own = a.lse + (size_t)T * Hq;
-    a.scale = scale, a.T = T, a.Hq = Hq, a.Hk = Hk, a.cap = cap, a.hs = hs, a.rs = rs;
+    a.scale = scale, a.T = T, a.Hq = Hq, a.Hk = Hk, a.cap = cap, a.ctas = long_ctas(), a.hs = hs, a.rs = rs;
+    a.part_o = static_cast<float*>(workspace), a.part_ml = reinterpret_cast<float2*>(a.part_o + part_rows(T, Hq) * D);
+    a.lse = reinterpret_cast<float*>(a.part_ml + part_rows(T, Hq)), a.own = a.lse + (size_t)T * Hq;
     return D == 64 ? launch_long_g<64>(a, static_cast<cudaStream_t>(stream)) : launch_long_g<128>(a, static_cast<cudaStream_t>(stream));
 }
