@@ -27,31 +27,34 @@ struct LongArgs {
     float* totals;       // [Hk, ts] what each logical row has been given, or null
     float* lse;          // [T, Hq] log2 of a row's denominator
     float* own;          // [T, Hq, 32] the scores of the pass's own rows in log2 units, -inf where not seen
-    float2* part_ml;     // a part's rows: maximum and sum ...
+    float* scores;       // [Hq, T, score_n] the scores of all keys in log2 units (passes of few rows), or null
+    float2* part_ml;     // a part's rows, then the units': maximum and sum ...
     float* part_o;       // ... and output [., D], not yet divided
+    long long unit_row;  // the units' first row: unit u of kv head g at unit_row + (g * units + u) * G
+    long long score_n;
     float scale;
     int T, Hq, Hk, win, cap, ctas;
     long long hs, rs, ts;
 };
 
 // ---- the pass's work, from what stands on the card ------------------------------------------------------------------
-// Key tiles of 128 rows. Per kv head there is an item for each prefix that rows share - its queries are all of those rows' -
-// and, in the rows layout, one for each row's own steps as far as they fill whole tiles; the rest of a row's own (fewer
-// than 128 steps, or a chain or tree pass's at most 32 rows) is the joining kernel's. The tiles of all heads in one line
-// are cut evenly over the CTAs; a CTA's stretch of an item is a part, whose state (maximum, sum, output row) the joining
-// kernel folds with the others'. Part (CTA c, item i) keeps its rows at c * T G + the rows of all items before i, which no
-// two parts share.
+// The prefixes: per kv head an item for each prefix that rows share, its queries all of those rows', its keys cut into
+// tiles of 128. The tiles of all heads in one line are cut evenly over the CTAs; a CTA's stretch of an item is a part, whose
+// state (maximum, sum, output row) the joining kernel folds with the others'. Part (CTA c, item i) keeps its rows at
+// c * T G + the rows of all items before i, which no two parts share.
+// A row's own keys (its steps in the rows layout, its path in a chain or tree pass) are no one else's: units of up to
+// `chunk` keys of one (row, kv head), a warp each, beside the tiles. A one-row pass's own key joins its prefix.
 constexpr int KT = 128;        // keys a tile
 constexpr int CTAS_MAX = 160;  // CTAs of the tile kernel at most
+constexpr int OWN_WARPS = 2;   // warps of a CTA that take units (two more would leave all of them 128 registers)
 
 struct Plan {
-    int mask[32];                               // item of lane l's prefix: its rows (0: no item)
-    int p_start[32], p_count[32];               // ... its first key (cache row, or logical row of a chain or tree pass) and keys
-    int p_tiles[32], p_tile0[32], p_row0[32];   // ... tiles, tiles and partial rows before it (within a kv head)
-    int s_start[32], s_tiles[32], s_tile0[32], s_row0[32];  // the same of row l's own steps
-    int lead[32];                               // row t's prefix item, -1: padding or refused
-    int own[32], own_n[32];                     // its remaining steps: the first's cache row, how many
-    int W, tiles, rows, n0;                     // ... and the kv head's tiles and partial rows
+    int mask[32];                             // item of lane l's prefix: its rows (0: no item)
+    int p_start[32], p_count[32];             // ... its first key (cache row, or logical row of a chain or tree pass) and keys
+    int p_tiles[32], p_tile0[32], p_row0[32]; // ... tiles, tiles and partial rows before it (within a kv head)
+    int lead[32];                             // row t's prefix item, -1: padding or refused
+    int own[32], own_n[32], unit0[32];        // its own keys: the first's cache row (rows layout), how many; units before it
+    int W, tiles, rows, units, chunk, n0;     // ... and the kv head's tiles, partial rows and units
 };
 
 __device__ __forceinline__ int warp_excl(int v, int lane, int& total) {
@@ -65,17 +68,32 @@ __device__ __forceinline__ int warp_excl(int v, int lane, int& total) {
     return x - v;
 }
 
+// units of a (row, kv head) at most: enough for every warp where rows and heads are few
+__host__ __device__ __forceinline__ int units_max(int T, int Hk) { return max(16, min(64, 1024 / (T * Hk))); }
+
 // one warp fills `P`; `tell`: this block records a refused layout
 __device__ __forceinline__ void make_plan(const LongArgs& A, int G, Plan& P, bool tell) {
     const int t = threadIdx.x & 31;
-    int mask = 0, start = 0, count = 0, s_start = 0, s_tiles = 0, lead = -1, own = 0, own_n = 0, W = 0, n0 = 0;
+    int mask = 0, start = 0, count = 0, lead = -1, own = 0, own_n = 0, W = 0, n0 = 0;
     if (A.rw == nullptr) {
         n0 = *A.n0p;
+        const int par = t < A.T ? A.par[t] : -1;
         if (n0 < 0 || n0 > A.cap - A.T) {
             if (tell && t == 0) b2_fail(B2_ERR_DOMAIN);
         } else {
             lead = t < A.T ? 0 : -1;
-            if (t == 0) mask = A.T == 32 ? -1 : (1 << A.T) - 1, count = n0;
+            if (t == 0) mask = A.T == 32 ? -1 : (1 << A.T) - 1, count = n0 + (A.T == 1);
+            if (A.T > 1) {  // the row's path as a set of the pass's rows
+                unsigned path = 0;
+                int q = t < A.T ? t : -1;
+                for (int k = 0; k < A.T; ++k) {
+                    const bool on = q >= 0 && q < A.T;
+                    if (on) path |= 1u << q;
+                    const int up = __shfl_sync(0xffffffffu, par, on ? q : 0);
+                    q = on ? up : -1;
+                }
+                own = (int)path, own_n = t < A.T ? __popc(path) : 0;
+            }
         }
     } else {
         const int base = A.rw[0], step = A.rw[1];
@@ -96,20 +114,22 @@ __device__ __forceinline__ void make_plan(const LongArgs& A, int G, Plan& P, boo
         if (live) {
             lead = __ffs(same) - 1;
             if (lead == t) mask = same, start = off + first, count = max(0, len - first);
-            const int i0 = max(0, first - len), n = step + 1 - i0;
-            s_start = base + i0 * W + col;
-            s_tiles = n / KT;
-            own = s_start + s_tiles * KT * W, own_n = n - s_tiles * KT;
+            const int i0 = max(0, first - len);
+            own = base + i0 * W + col, own_n = step + 1 - i0;
         }
     }
     const int p_tiles = mask ? (count + KT - 1) / KT : 0;
-    int pt, st, pr, sr;
-    const int p_tile0 = warp_excl(p_tiles, t, pt), s_tile0 = warp_excl(s_tiles, t, st);
-    const int p_row0 = warp_excl(p_tiles ? __popc(mask) * G : 0, t, pr), s_row0 = warp_excl(s_tiles ? G : 0, t, sr);
+    int pt, pr, keys, units;
+    const int p_tile0 = warp_excl(p_tiles, t, pt), p_row0 = warp_excl(p_tiles ? __popc(mask) * G : 0, t, pr);
+    // units of about a warp's fair share of the own keys, a multiple of 32, no row in more of them than its room allows
+    (void)warp_excl(min(own_n, 1 << 20), t, keys);
+    int chunk = (int)(((long long)keys * A.Hk + A.ctas * OWN_WARPS - 1) / (A.ctas * OWN_WARPS));
+    const int most = __reduce_max_sync(0xffffffffu, own_n), room = units_max(A.T, A.Hk);
+    chunk = (max(chunk, (most + room - 1) / room) + 31) & ~31;
+    const int unit0 = warp_excl(own_n > 0 ? (own_n + chunk - 1) / chunk : 0, t, units);
     P.mask[t] = mask, P.p_start[t] = start, P.p_count[t] = count, P.p_tiles[t] = p_tiles, P.p_tile0[t] = p_tile0, P.p_row0[t] = p_row0;
-    P.s_start[t] = s_start, P.s_tiles[t] = s_tiles, P.s_tile0[t] = pt + s_tile0, P.s_row0[t] = pr + s_row0;
-    P.lead[t] = lead, P.own[t] = own, P.own_n[t] = own_n;
-    if (t == 0) P.W = W, P.tiles = pt + st, P.rows = pr + sr, P.n0 = n0;
+    P.lead[t] = lead, P.own[t] = own, P.own_n[t] = own_n, P.unit0[t] = unit0;
+    if (t == 0) P.W = W, P.tiles = pt, P.rows = pr, P.units = units, P.chunk = chunk, P.n0 = n0;
     __syncwarp();
 }
 
@@ -122,10 +142,9 @@ __device__ __forceinline__ long long first_tile(long long tiles, int c, int ctas
 
 // a CTA's stretch of one item
 struct Part {
-    int head, mask, start, stride, keys, tiles, rows;  // `keys`: of these tiles (the last may be partly filled)
-    long long row0;                                    // its first partial row
-    long long end;                                     // the first tile past it
-    bool prefix;
+    int head, mask, start, keys, tiles, rows;  // `keys`: of these tiles (the last may be partly filled)
+    long long row0;                            // its first partial row
+    long long end;                             // the first tile past it
 };
 // the part that begins at tile `at` of a CTA whose stretch ends at `stop` (every lane of a warp asks alike)
 __device__ __forceinline__ Part part_at(const Plan& P, const LongArgs& A, int G, long long at, long long stop, int cta) {
@@ -133,19 +152,14 @@ __device__ __forceinline__ Part part_at(const Plan& P, const LongArgs& A, int G,
     Part p;
     p.head = (int)(at / P.tiles);
     const int in = (int)(at - (long long)p.head * P.tiles);
-    const unsigned pp = __ballot_sync(0xffffffffu, in >= P.p_tile0[lane] && in < P.p_tile0[lane] + P.p_tiles[lane]);
-    const unsigned ss = __ballot_sync(0xffffffffu, in >= P.s_tile0[lane] && in < P.s_tile0[lane] + P.s_tiles[lane]);
-    p.prefix = pp != 0;
-    const int l = __ffs(p.prefix ? pp : ss) - 1;
-    const int tile0 = p.prefix ? P.p_tile0[l] : P.s_tile0[l], tiles = p.prefix ? P.p_tiles[l] : P.s_tiles[l];
-    const int skip = in - tile0;
-    p.tiles = (int)min((long long)(tiles - skip), stop - at);
-    p.mask = p.prefix ? P.mask[l] : 1 << l;
-    p.stride = p.prefix ? 1 : P.W;
-    p.start = (p.prefix ? P.p_start[l] : P.s_start[l]) + skip * KT * p.stride;
-    p.keys = min(p.tiles * KT, (p.prefix ? P.p_count[l] : tiles * KT) - skip * KT);
+    const int l = __ffs(__ballot_sync(0xffffffffu, in >= P.p_tile0[lane] && in < P.p_tile0[lane] + P.p_tiles[lane])) - 1;
+    const int skip = in - P.p_tile0[l];
+    p.tiles = (int)min((long long)(P.p_tiles[l] - skip), stop - at);
+    p.mask = P.mask[l];
+    p.start = P.p_start[l] + skip * KT;
+    p.keys = min(p.tiles * KT, P.p_count[l] - skip * KT);
     p.rows = __popc(p.mask) * G;
-    p.row0 = (long long)cta * A.T * G + (long long)p.head * P.rows + (p.prefix ? P.p_row0[l] : P.s_row0[l]);
+    p.row0 = (long long)cta * A.T * G + (long long)p.head * P.rows + P.p_row0[l];
     p.end = at + p.tiles;
     return p;
 }
@@ -232,7 +246,7 @@ __device__ __forceinline__ void tma_rows4(uint32_t dst, const CUtensorMap* tm, i
         : "memory");
 }
 
-constexpr int TW = 10;          // warps: two warpgroups for the weights, the loads' warp, the MMAs' warp
+constexpr int TW = 10 + OWN_WARPS;  // warps: two warpgroups for the weights, the loads' warp, the MMAs' warp, the units' warps
 constexpr int STAGES_MAX = 6;   // stages of a ring
 
 struct alignas(8) TileSync {
@@ -267,7 +281,118 @@ __device__ __forceinline__ bool wait_or_fail(uint64_t* bar, uint32_t parity, Til
     return __all_sync(0xffffffffu, ok);
 }
 
-template <int D>
+// a warp's units: every `stride`-th from `first` on. A lane a key for the scores and D / 32 dims for the output, a running
+// maximum and sum over 32 keys at a time; keys outside are never read.
+template <int D, int G>
+__device__ __forceinline__ void own_units(const LongArgs& A, const Plan& P, int first, int stride) {
+    constexpr int E = D / 32, VB = 16;
+    const int lane = threadIdx.x & 31;
+    const float scale2 = __fmul_rn(A.scale, LOG2E);
+    const long long all = (long long)P.units * A.Hk;
+    for (long long u = first; u < all; u += stride) {
+        const int g = (int)(u / P.units), in = (int)(u - (long long)g * P.units);
+        const int t = 31 - __clz(__ballot_sync(0xffffffffu, P.own_n[lane] > 0 && P.unit0[lane] <= in));
+        const int i0 = (in - P.unit0[t]) * P.chunk, n = min(P.chunk, P.own_n[t] - i0), own = P.own[t];
+        const bf16* Kg = A.K + (size_t)g * A.hs;
+        const bf16* Vg = A.V + (size_t)g * A.hs;
+        const uint4* q = reinterpret_cast<const uint4*>(A.q + ((size_t)t * A.Hq + g * G) * D);
+        float m[G], l[G], o[G][E];
+#pragma unroll
+        for (int hh = 0; hh < G; ++hh) {
+            m[hh] = NEG_INF, l[hh] = 0.f;
+#pragma unroll
+            for (int e = 0; e < E; ++e) o[hh][e] = 0.f;
+        }
+        for (int j0 = 0; j0 < n; j0 += 32) {
+            int row = -1;
+            if (j0 + lane < n) {
+                if (A.rw != nullptr) {
+                    row = own + (i0 + j0 + lane) * P.W;
+                } else {
+                    row = P.n0 + (int)__fns((unsigned)own, 0, j0 + lane + 1);
+                    if (A.tbl != nullptr) row = A.tbl[row];
+                    if (row < 0 || row >= A.cap) {
+                        b2_fail(B2_ERR_DOMAIN);
+                        row = -1;
+                    }
+                }
+            }
+            float s[G];
+#pragma unroll
+            for (int hh = 0; hh < G; ++hh) s[hh] = 0.f;
+            const uint4* kr = reinterpret_cast<const uint4*>(Kg + (size_t)max(row, 0) * A.rs);
+#pragma unroll
+            for (int c0 = 0; c0 < D / 8; c0 += 8) {
+                uint4 kv[8];
+#pragma unroll
+                for (int c = 0; c < 8; ++c) kv[c] = row >= 0 ? __ldg(kr + c0 + c) : make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+                for (int c = 0; c < 8; ++c)
+#pragma unroll
+                    for (int hh = 0; hh < G; ++hh) {
+                        const uint4 w = __ldg(q + hh * (D / 8) + c0 + c);
+                        s[hh] = fma2_bf16(kv[c].w, w.w, fma2_bf16(kv[c].z, w.z, fma2_bf16(kv[c].y, w.y, fma2_bf16(kv[c].x, w.x, s[hh]))));
+                    }
+            }
+#pragma unroll
+            for (int hh = 0; hh < G; ++hh) {
+                s[hh] = row >= 0 ? __fmul_rn(s[hh], scale2) : NEG_INF;
+                if (A.own != nullptr) {
+                    const bool on = ((unsigned)own >> lane) & 1u;
+                    const float v = __shfl_sync(0xffffffffu, s[hh], __popc((unsigned)own & ((1u << lane) - 1u)));
+                    A.own[((size_t)t * A.Hq + g * G + hh) * 32 + lane] = on ? v : NEG_INF;
+                }
+                float mx = s[hh];
+#pragma unroll
+                for (int k = 16; k > 0; k >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, k));
+                mx = fmaxf(mx, m[hh]);
+                const float c = m[hh] == NEG_INF ? 0.f : ex2(m[hh] - mx);
+                const float p = s[hh] == NEG_INF ? 0.f : ex2(s[hh] - mx);
+                l[hh] = l[hh] * c + warp_sum(p);
+                m[hh] = mx;
+                s[hh] = p;
+#pragma unroll
+                for (int e = 0; e < E; ++e) o[hh][e] *= c;
+            }
+#pragma unroll 1
+            for (int k0 = 0; k0 < 32; k0 += VB) {
+                if (k0 >= n - j0) break;
+                unsigned short v[VB][E];
+#pragma unroll
+                for (int k = 0; k < VB; ++k) {  // (a key outside has weight 0 over zeros)
+                    const int r = __shfl_sync(0xffffffffu, row, k0 + k);
+                    const bf16* vr = Vg + (size_t)max(r, 0) * A.rs + lane * E;
+                    if (E == 4) {
+                        const uint2 x = r >= 0 ? __ldg(reinterpret_cast<const uint2*>(vr)) : make_uint2(0u, 0u);
+                        split_bf16(x.x, v[k][0], v[k][1]);
+                        split_bf16(x.y, v[k][E - 2], v[k][E - 1]);
+                    } else {
+                        const uint32_t x = r >= 0 ? __ldg(reinterpret_cast<const uint32_t*>(vr)) : 0u;
+                        split_bf16(x, v[k][0], v[k][E - 1]);
+                    }
+                }
+#pragma unroll
+                for (int k = 0; k < VB; ++k)
+#pragma unroll
+                    for (int hh = 0; hh < G; ++hh) {
+                        const float p = __shfl_sync(0xffffffffu, s[hh], k0 + k);
+#pragma unroll
+                        for (int e = 0; e < E; ++e) o[hh][e] = fmaf(p, __uint_as_float((uint32_t)v[k][e] << 16), o[hh][e]);
+                    }
+            }
+        }
+        const size_t at = (size_t)(A.unit_row + u * G);
+#pragma unroll
+        for (int hh = 0; hh < G; ++hh) {
+            if (lane == 0) A.part_ml[at + hh] = make_float2(m[hh], l[hh]);
+            float* to = A.part_o + (at + hh) * D + lane * E;
+            if (E == 4) *reinterpret_cast<float4*>(to) = make_float4(o[hh][0], o[hh][1], o[hh][E - 2], o[hh][E - 1]);
+            else *reinterpret_cast<float2*>(to) = make_float2(o[hh][0], o[hh][E - 1]);
+        }
+    }
+}
+
+template <int D, int G>
 __global__ void __launch_bounds__(TW * 32, 1)
     long_tiles(const __grid_constant__ CUtensorMap kbox, const __grid_constant__ CUtensorMap krows,
                const __grid_constant__ CUtensorMap vbox, const __grid_constant__ CUtensorMap vrows, const TileArgs X) {
@@ -280,12 +405,9 @@ __global__ void __launch_bounds__(TW * 32, 1)
     __shared__ float s_m[128], s_l[128];
     uint8_t* smem = smem_raw;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int G = A.Hq / A.Hk, nq = A.T * G > 128 ? 2 : 1;
+    const int nq = A.T * G > 128 ? 2 : 1;
     const uint32_t sq = smem_u32(smem), sk = sq + nq * TILE, sv = sk + X.ks * TILE;
 
-    pdl_launch_dependents();
-    pdl_wait();
-    if (warp == 0) make_plan(A, G, plan, blockIdx.x == 0);
     if (threadIdx.x == 32) {
         for (int s = 0; s < STAGES_MAX; ++s) {
             mbar_init(smem_u32(&sy.kfull[s]), 1), mbar_init(smem_u32(&sy.kempty[s]), 1);
@@ -298,10 +420,17 @@ __global__ void __launch_bounds__(TW * 32, 1)
         sy.fail = 0;
         mbar_fence_init();
     }
+    // the kernels before are through; only now may the joining kernel start, which reads what they left before it waits
+    pdl_wait();
+    pdl_launch_dependents();
+    if (warp == 0) make_plan(A, G, plan, blockIdx.x == 0);
     __syncthreads();
     const long long all = (long long)plan.tiles * A.Hk;
     const long long begin = first_tile(all, blockIdx.x, gridDim.x), stop = first_tile(all, blockIdx.x + 1, gridDim.x);
-    if (begin >= stop) return;  // (no work for this CTA: nothing allocated yet)
+    if (begin >= stop) {  // no tiles for this CTA: nothing allocated yet
+        if (warp >= 10) own_units<D, G>(A, plan, (warp - 10) * gridDim.x + blockIdx.x, OWN_WARPS * gridDim.x);
+        return;
+    }
     if (sq & 1023) {  // (the tiles take all but 3 KB of what a block may have: there is no room to align them here)
         if (threadIdx.x == 0) b2_fail(B2_ERR_CUDA);
         return;
@@ -391,6 +520,9 @@ __global__ void __launch_bounds__(TW * 32, 1)
                     m = ref;
                     const float sub = m == NEG_INF ? 0.f : m;
                     float sum[4] = {0.f, 0.f, 0.f, 0.f};
+                    float* keep = nullptr;  // where this row's scores go
+                    if (A.scores != nullptr && row < valid)
+                        keep = A.scores + ((size_t)p.head * p.rows + row) * A.score_n + p.start + (size_t)(two ? i : 2 * i + wg) * KT;
 #pragma unroll
                     for (int c0 = 0; c0 < KT; c0 += 32) {
                         uint32_t(&v)[32] = s[(c0 >> 5) & 1];
@@ -409,6 +541,13 @@ __global__ void __launch_bounds__(TW * 32, 1)
                             asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w[c]) : "f"(b), "f"(a));
                         }
                         tm_st16(ts + c0 / 2, w);
+                        if (keep != nullptr) {
+#pragma unroll
+                            for (int c = 0; c < 32; c += 4)
+                                *reinterpret_cast<float4*>(keep + c0 + c) =
+                                    make_float4(__uint_as_float(v[c]) * scale2, __uint_as_float(v[c + 1]) * scale2,
+                                                __uint_as_float(v[c + 2]) * scale2, __uint_as_float(v[c + 3]) * scale2);
+                        }
                     }
                     l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
                     tm_wait_st();
@@ -483,10 +622,10 @@ __global__ void __launch_bounds__(TW * 32, 1)
             const Part p = part_at(plan, A, G, at, stop, blockIdx.x);
             at = p.end;
             const int x = p.head * X.col_mul, y0 = p.head * X.row_mul;
-            const bool mapped = p.prefix && A.tbl != nullptr;
+            const bool mapped = A.tbl != nullptr;
             for (int i = 0; i < p.tiles && ok; ++i) {
                 const int keys = min(KT, p.keys - i * KT);
-                const bool box = keys == KT && p.stride == 1 && !mapped;
+                const bool box = keys == KT && !mapped;
                 int y[4];
                 if (box) {
                     y[0] = y0 + p.start + i * KT;
@@ -495,7 +634,7 @@ __global__ void __launch_bounds__(TW * 32, 1)
                     // values multiplied by it must be ones that the rows see)
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {
-                        const int j = p.start + (i * KT + min(lane * 4 + k, keys - 1)) * p.stride;
+                        const int j = p.start + i * KT + min(lane * 4 + k, keys - 1);
                         int r = mapped ? A.tbl[j] : j;
                         if (r < 0 || r >= A.cap) {
                             b2_fail(B2_ERR_DOMAIN);
@@ -537,6 +676,8 @@ __global__ void __launch_bounds__(TW * 32, 1)
             const long long uses = vn / X.vs + (s < vn % X.vs ? 1 : 0);
             if (uses > 0) (void)mbar_wait_bounded(smem_u32(&sy.vfull[s]), (uint32_t)(uses - 1) & 1);
         }
+    } else if (warp >= 10) {
+        own_units<D, G>(A, plan, (warp - 10) * gridDim.x + blockIdx.x, OWN_WARPS * gridDim.x);
     } else {
         // ---- the MMAs -----------------------------------------------------------------------------------------------------------
         // D f32, A and B bf16; S: both K-major, N = 128 keys; O: the values' dims are B's N and lie contiguous, N = D
@@ -604,187 +745,140 @@ __global__ void __launch_bounds__(TW * 32, 1)
 }
 
 // ---- a row's parts joined ------------------------------------------------------------------------------------------------
-constexpr int JW = KT / 32;                    // warps of a row's block
-constexpr int PARTS_MAX = 2 * (CTAS_MAX + 1);  // parts of a row's prefix and own steps
+constexpr int JT = 256, JW = JT / 32;      // threads and warps of a block
+constexpr int STATES_MAX = CTAS_MAX + 64;  // a row's parts and units
+constexpr int KEEP_ROWS = 16;              // a kv head's queries (T G) up to which a pass keeps its scores for the weights
 
-// One block a (row, kv head): its warps take the row's remaining own keys 32 at a time (a lane a key for the scores, D / 32
-// dims for the output; keys outside are never touched), then their states, the parts' and the sink are folded.
-template <int D, int G>
-__global__ void __launch_bounds__(JW * 32) long_join(const LongArgs A) {
-    constexpr int E = D / 32;
-    __shared__ Plan plan;
-    __shared__ __align__(16) uint32_t qs[G][D / 2];
-    __shared__ float ps[JW][G][32];
-    __shared__ float wm[JW][G], wl[JW][G];
-    __shared__ float wo[JW][G][D];
-    __shared__ float fac[G][PARTS_MAX];
-    __shared__ float top[G], den[G];
-    __shared__ int anc[TMAX];
-    __shared__ int s_len;
-    pdl_launch_dependents();
-    pdl_wait();
-    const int t = blockIdx.x, g = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    if (warp == 0) make_plan(A, G, plan, false);
-    if (threadIdx.x == 32) {
-        int len = 0;
-        if (A.rw == nullptr) {
-            for (int p = t; p >= 0 && p < A.T && len < TMAX; p = A.par[p]) ++len;
-            int k = len;
-            for (int p = t; k > 0; p = A.par[p]) anc[--k] = p;
+// where the states of (row t, kv head g) lie: state k of query head hh in row at(k) + hh
+struct States {
+    long long p_row, u_row;
+    int np, n, step, G;
+    __device__ __forceinline__ States(const LongArgs& A, const Plan& P, int t, int g, int G_) : G(G_) {
+        const int lead = P.lead[t];
+        const long long all = (long long)P.tiles * A.Hk, tile = (long long)g * P.tiles + P.p_tile0[lead];
+        int c = 0;
+        np = 0, step = A.T * G;
+        if (P.p_tiles[lead] > 0) {
+            c = cta_of(A, all, tile);
+            np = cta_of(A, all, tile + P.p_tiles[lead] - 1) - c + 1;
         }
-        s_len = len;
+        const int below = __popc(P.mask[lead] & ((1u << t) - 1u));  // the row's place among its prefix's
+        p_row = (long long)c * step + (long long)g * P.rows + P.p_row0[lead] + below * G;
+        u_row = A.unit_row + ((long long)g * P.units + P.unit0[t]) * G;
+        n = np + (P.own_n[t] > 0 ? (P.own_n[t] + P.chunk - 1) / P.chunk : 0);
     }
-    for (int i = threadIdx.x; i < G * D / 2; i += JW * 32) {
-        const int hh = i / (D / 2), d = i - hh * (D / 2);
-        qs[hh][d] = reinterpret_cast<const uint32_t*>(A.q + ((size_t)t * A.Hq + g * G + hh) * D)[d];
-    }
-    if (A.own != nullptr)
-        for (int i = threadIdx.x; i < G * 32; i += JW * 32) A.own[((size_t)t * A.Hq + g * G) * 32 + i] = NEG_INF;
-    __syncthreads();
-    const int lead = plan.lead[t];
-    if (lead < 0) return;  // padding, or refused
-    const int n = A.rw != nullptr ? plan.own_n[t] : s_len;
-    const float scale2 = __fmul_rn(A.scale, LOG2E);
-    const bf16* Kg = A.K + (size_t)g * A.hs;
-    const bf16* Vg = A.V + (size_t)g * A.hs;
-    float m[G], l[G], o[G][E];
-#pragma unroll
-    for (int hh = 0; hh < G; ++hh) {
-        m[hh] = NEG_INF, l[hh] = 0.f;
-#pragma unroll
-        for (int e = 0; e < E; ++e) o[hh][e] = 0.f;
-    }
-    const int i = warp * 32 + lane;  // (at most 127 keys: a warp's one stretch)
-    if (warp * 32 < n) {
-        int row = -1;
-        if (i < n) {
-            if (A.rw != nullptr) {
-                row = plan.own[t] + i * plan.W;
-            } else {
-                row = plan.n0 + anc[i];
-                if (A.tbl != nullptr) row = A.tbl[row];
-                if (row < 0 || row >= A.cap) {
-                    b2_fail(B2_ERR_DOMAIN);
-                    row = -1;
-                }
-            }
-        }
-        float s[G];
-#pragma unroll
-        for (int hh = 0; hh < G; ++hh) s[hh] = 0.f;
-        if (row >= 0) {
-            const uint4* kr = reinterpret_cast<const uint4*>(Kg + (size_t)row * A.rs);
-#pragma unroll 8
-            for (int c = 0; c < D / 8; ++c) {
-                const uint4 kv = __ldg(kr + c);
-#pragma unroll
-                for (int hh = 0; hh < G; ++hh) {
-                    const uint4 q4 = *reinterpret_cast<const uint4*>(&qs[hh][c * 4]);
-                    s[hh] = fma2_bf16(kv.w, q4.w, fma2_bf16(kv.z, q4.z, fma2_bf16(kv.y, q4.y, fma2_bf16(kv.x, q4.x, s[hh]))));
-                }
-            }
-        }
-#pragma unroll
-        for (int hh = 0; hh < G; ++hh) {
-            s[hh] = row >= 0 ? __fmul_rn(s[hh], scale2) : NEG_INF;
-            if (A.own != nullptr && i < n) A.own[((size_t)t * A.Hq + g * G + hh) * 32 + anc[i]] = s[hh];
-            float mx = s[hh];
-#pragma unroll
-            for (int k = 16; k > 0; k >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, k));
-            const float p = s[hh] == NEG_INF ? 0.f : ex2(s[hh] - mx);
-            l[hh] = warp_sum(p);
-            m[hh] = mx;
-            ps[warp][hh][lane] = p;
-        }
-        __syncwarp();
-        for (int k = 0; k < 32; ++k) {
-            const int r = __shfl_sync(0xffffffffu, row, k);
-            if (r < 0) continue;
-            __align__(8) bf16 v[E];
-            ld_run<E, false>(Vg + (size_t)r * A.rs + lane * E, v);
-#pragma unroll
-            for (int hh = 0; hh < G; ++hh)
-#pragma unroll
-                for (int e = 0; e < E; ++e) o[hh][e] = fmaf(ps[warp][hh][k], bf2f(v[e]), o[hh][e]);
-        }
-    }
-#pragma unroll
-    for (int hh = 0; hh < G; ++hh) {
-        if (lane == 0) wm[warp][hh] = m[hh], wl[warp][hh] = l[hh];
-#pragma unroll
-        for (int e = 0; e < E; ++e) wo[warp][hh][lane * E + e] = o[hh][e];
-    }
-    // the parts: those of the prefix's item, then those of the row's own steps; part k of an item is the k-th CTA's that
-    // holds tiles of it
-    const long long all = (long long)plan.tiles * A.Hk, head0 = (long long)g * plan.tiles, row_g = (long long)g * plan.rows;
-    int np = 0, ns = 0, pc = 0, sc = 0;
-    auto cta_of = [&](long long tile) {  // the CTA whose stretch holds `tile`
+    // the CTA whose stretch holds `tile`
+    static __device__ __forceinline__ int cta_of(const LongArgs& A, long long all, long long tile) {
         int c = (int)(tile * min((long long)A.ctas, all) / all);
         while (first_tile(all, c, A.ctas) > tile) --c;
         while (first_tile(all, c + 1, A.ctas) <= tile) ++c;
         return c;
-    };
-    if (plan.p_tiles[lead] > 0) {
-        pc = cta_of(head0 + plan.p_tile0[lead]);
-        np = cta_of(head0 + plan.p_tile0[lead] + plan.p_tiles[lead] - 1) - pc + 1;
     }
-    if (plan.s_tiles[t] > 0) {
-        sc = cta_of(head0 + plan.s_tile0[t]);
-        ns = cta_of(head0 + plan.s_tile0[t] + plan.s_tiles[t] - 1) - sc + 1;
-    }
-    const int below = __popc(plan.mask[lead] & ((1u << t) - 1u));  // the row's place among its prefix's
-    auto part_row = [&](int k) {
-        return k < np ? (long long)(pc + k) * A.T * G + row_g + plan.p_row0[lead] + below * G
-                      : (long long)(sc + k - np) * A.T * G + row_g + plan.s_row0[t];
-    };
-    __syncthreads();
-    for (int hh = warp; hh < G; hh += JW) {  // a warp a head: the largest maximum, each state's factor, the sum
-        float M = lane < JW ? wm[lane][hh] : NEG_INF;
-        for (int k = lane; k < np + ns; k += 32) M = fmaxf(M, A.part_ml[part_row(k) + hh].x);
-        const float sink = A.sinks != nullptr ? __fmul_rn(A.sinks[g * G + hh], LOG2E) : NEG_INF;
-        M = fmaxf(M, sink);
+    __device__ __forceinline__ long long at(int k) const { return k < np ? p_row + (long long)k * step : u_row + (long long)(k - np) * G; }
+};
+// a warp's look at a query head's states: the largest maximum M and the sum L relative to it, the sink in both; the states'
+// factors into `fac` where given
+__device__ __forceinline__ void row_stats(const LongArgs& A, const States& S, int head, int hh, float& M, float& L, float* fac) {
+    const int lane = threadIdx.x & 31;
+    const float sink = A.sinks != nullptr ? __fmul_rn(A.sinks[head], LOG2E) : NEG_INF;
+    M = sink;
+    for (int k = lane; k < S.n; k += 32) M = fmaxf(M, A.part_ml[S.at(k) + hh].x);
 #pragma unroll
-        for (int k = 16; k > 0; k >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, k));
-        const float sub = M == NEG_INF ? 0.f : M;
-        float L = 0.f;
-        if (lane < JW) {
-            const float f = wm[lane][hh] == NEG_INF ? 0.f : ex2(wm[lane][hh] - sub);
-            L += f * wl[lane][hh];
-            wm[lane][hh] = f;
+    for (int k = 16; k > 0; k >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, k));
+    const float sub = M == NEG_INF ? 0.f : M;
+    L = 0.f;
+    for (int k = lane; k < S.n; k += 32) {
+        const float2 ml = A.part_ml[S.at(k) + hh];
+        const float f = ml.x == NEG_INF ? 0.f : ex2(ml.x - sub);
+        L += f * ml.y;
+        if (fac != nullptr) fac[k] = f;
+    }
+    L = warp_sum(L);
+    if (A.sinks != nullptr) L += ex2(sink - sub);
+}
+
+// The first T Hq blocks join one (row, query head) each: a warp every eighth state, a lane D / 32 dims, the warps' sums added
+// in order. The blocks after them, where a pass of few rows kept its scores, add up what it gives each cache row: a thread
+// a key, 2^(score - log2 of the row's denominator) over the kv head's queries in order - one sum in one order.
+template <int D, int G>
+__global__ void __launch_bounds__(JT) long_join(const LongArgs A, int weight_blocks) {
+    constexpr int E = D / 32;
+    __shared__ Plan plan;
+    __shared__ float fac[STATES_MAX];
+    __shared__ float part[JW][D];
+    __shared__ float s_lse[KEEP_ROWS];
+    __shared__ float s_den;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    pdl_launch_dependents();
+    if (warp == 0) make_plan(A, G, plan, false);
+    __syncthreads();
+    if ((int)blockIdx.x < A.T * A.Hq) {
+        const int t = blockIdx.x / A.Hq, head = blockIdx.x - t * A.Hq, g = head / G, hh = head - g * G;
+        if (plan.lead[t] < 0) {  // padding, or refused
+            pdl_wait();
+            return;
         }
-        for (int k = lane; k < np + ns; k += 32) {
-            const float2 ml = A.part_ml[part_row(k) + hh];
-            const float f = ml.x == NEG_INF ? 0.f : ex2(ml.x - sub);
-            L += f * ml.y;
-            fac[hh][k] = f;
+        const States S(A, plan, t, g, G);
+        pdl_wait();
+        if (warp == 0) {
+            float M, L;
+            row_stats(A, S, head, hh, M, L, fac);
+            if (lane == 0) {
+                s_den = L;
+                if (A.lse != nullptr) A.lse[(size_t)t * A.Hq + head] = M + log2f(L);
+            }
         }
-        L = warp_sum(L);
-        if (lane == 0) {
-            if (A.sinks != nullptr) L += ex2(sink - sub);
-            top[hh] = M, den[hh] = L;
+        __syncthreads();
+        float o[E];
+#pragma unroll
+        for (int e = 0; e < E; ++e) o[e] = 0.f;
+#pragma unroll 4
+        for (int k = warp; k < S.n; k += JW) {
+            const float f = fac[k];
+            const float* src = A.part_o + (size_t)(S.at(k) + hh) * D + lane * E;
+            if (E == 4) {
+                const float4 v = *reinterpret_cast<const float4*>(src);
+                o[0] = fmaf(f, v.x, o[0]), o[1] = fmaf(f, v.y, o[1]), o[E - 2] = fmaf(f, v.z, o[E - 2]), o[E - 1] = fmaf(f, v.w, o[E - 1]);
+            } else {
+                const float2 v = *reinterpret_cast<const float2*>(src);
+                o[0] = fmaf(f, v.x, o[0]), o[E - 1] = fmaf(f, v.y, o[E - 1]);
+            }
         }
+#pragma unroll
+        for (int e = 0; e < E; ++e) part[warp][lane * E + e] = o[e];
+        __syncthreads();
+        if (threadIdx.x < D) {
+            float a = 0.f;
+            for (int w = 0; w < min(JW, S.n); ++w) a += part[w][threadIdx.x];
+            A.out[(size_t)blockIdx.x * D + threadIdx.x] = f2bf(__fdiv_rn(a, s_den));
+        }
+        return;
+    }
+    // ---- the weights ------------------------------------------------------------------------------------------------------
+    const int b = blockIdx.x - A.T * A.Hq, g = b / weight_blocks, n = plan.n0 + (A.T == 1);  // keys whose scores were kept
+    int j = (b - g * weight_blocks) * JT + threadIdx.x;
+    pdl_wait();
+    if (plan.lead[0] < 0 || (j - (int)threadIdx.x >= n && b != g * weight_blocks)) return;
+    for (int r = warp; r < A.T * G; r += JW) {
+        const int t = r / G, hh = r - t * G;
+        const States S(A, plan, t, g, G);
+        float M, L;
+        row_stats(A, S, g * G + hh, hh, M, L, nullptr);
+        if (lane == 0) s_lse[r] = M + log2f(L);
     }
     __syncthreads();
-    for (int i4 = threadIdx.x; i4 < G * D / 4; i4 += JW * 32) {
-        const int hh = i4 / (D / 4), d = (i4 - hh * (D / 4)) * 4, head = g * G + hh;
-        float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int w = 0; w * 32 < n; ++w) {
-            const float f = wm[w][hh];
-            const float4 v = *reinterpret_cast<const float4*>(&wo[w][hh][d]);
-            O.x = fmaf(f, v.x, O.x), O.y = fmaf(f, v.y, O.y), O.z = fmaf(f, v.z, O.z), O.w = fmaf(f, v.w, O.w);
-        }
-#pragma unroll 4
-        for (int k = 0; k < np + ns; ++k) {
-            const float f = fac[hh][k];
-            const float4 v = *reinterpret_cast<const float4*>(A.part_o + (size_t)(part_row(k) + hh) * D + d);
-            O.x = fmaf(f, v.x, O.x), O.y = fmaf(f, v.y, O.y), O.z = fmaf(f, v.z, O.z), O.w = fmaf(f, v.w, O.w);
-        }
-        const float L = den[hh];
-        __nv_bfloat162 a, b;
-        a.x = f2bf(__fdiv_rn(O.x, L)), a.y = f2bf(__fdiv_rn(O.y, L)), b.x = f2bf(__fdiv_rn(O.z, L)), b.y = f2bf(__fdiv_rn(O.w, L));
-        __nv_bfloat162* out = reinterpret_cast<__nv_bfloat162*>(A.out + ((size_t)t * A.Hq + head) * D + d);
-        out[0] = a, out[1] = b;
-        if (d == 0 && A.lse != nullptr) A.lse[(size_t)t * A.Hq + head] = top[hh] + log2f(L);
+    float* tot = A.totals + (size_t)g * A.ts;
+    if (A.T > 1 && b == g * weight_blocks && (int)threadIdx.x < A.T) {  // the pass's own rows: set
+        float a = 0.f;
+        for (int r = 0; r < A.T * G; ++r)
+            a += ex2(A.own[((size_t)(r / G) * A.Hq + g * G + r % G) * 32 + threadIdx.x] - s_lse[r]);
+        tot[plan.n0 + threadIdx.x] = a;
+    }
+    for (; j < n; j += weight_blocks * JT) {
+        float a = 0.f;
+#pragma unroll 8
+        for (int r = 0; r < A.T * G; ++r) a += ex2(A.scores[((size_t)g * A.T * G + r) * A.score_n + j] - s_lse[r]);
+        tot[j] = j < plan.n0 ? tot[j] + a : a;
     }
 }
 
@@ -862,15 +956,37 @@ int make_map(CUtensorMap* tm, const void* base, long long rows, long long cols, 
                : B2_ERR_DOMAIN;
 }
 
-int long_ctas() { return min(b2_sm_count(), CTAS_MAX); }
-// partial rows at most: every CTA's stretch moves on by one item's rows, every kv head by its items'
-size_t part_rows(int T, int Hq) { return (size_t)long_ctas() * T * Hq + (size_t)2 * T * Hq; }
+// the kernels of a call start under programmatic dependent launch (bit 3 of the `pdl` tunable): each sets up while the one
+// before it drains
+template <typename... P, typename... A>
+int launch(void (*kern)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t s, const A&... args) {
+    cudaLaunchConfig_t cfg;
+    memset(&cfg, 0, sizeof cfg);
+    cfg.gridDim = grid, cfg.blockDim = block, cfg.dynamicSmemBytes = smem, cfg.stream = s;
+    cudaLaunchAttribute at[1];
+    if (b2_tuning().pdl & 8) {
+        at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        at[0].val.programmaticStreamSerializationAllowed = 1;
+        cfg.attrs = at, cfg.numAttrs = 1;
+    }
+    if (cudaLaunchKernelEx(&cfg, kern, args...) != cudaSuccess) {
+        (void)cudaGetLastError();
+        return B2_ERR_CUDA;
+    }
+    return B2_OK;
+}
 
-template <int D>
+int long_ctas() { return min(b2_sm_count(), CTAS_MAX); }
+// rows of the parts at most: every CTA's stretch moves on by one item's rows, every kv head by its items'
+size_t part_rows(int T, int Hq) { return (size_t)long_ctas() * T * Hq + (size_t)T * Hq; }
+size_t state_rows(int T, int Hq, int Hk) { return part_rows(T, Hq) + (size_t)T * Hq * units_max(T, Hk); }
+long long score_stride(int cap) { return ((long long)cap + KT - 1) / KT * KT; }
+bool keeps_scores(int T, int Hq, int Hk) { return T * (Hq / Hk) <= KEEP_ROWS; }
+
+template <int D, int G>
 int launch_tiles(const LongArgs& a, cudaStream_t s) {
     TileArgs x{};
     x.a = a;
-    const int G = a.Hq / a.Hk;
     const bool by_row = a.Hk == 1 || (a.Hk - 1) * a.hs + D <= a.rs;  // kv heads inside a cache row
     const long long rows = by_row ? a.cap : (a.Hk - 1) * (a.hs / a.rs) + a.cap, cols = by_row ? (a.Hk - 1) * (a.Hk > 1 ? a.hs : 0) + D : D;
     if (rows > 0x7fffffffLL || cols > 0x7fffffffLL) return B2_ERR_DOMAIN;
@@ -881,27 +997,22 @@ int launch_tiles(const LongArgs& a, cudaStream_t s) {
     const int tile = KT * D * 2, nq = a.T * G > 128 ? 2 : 1, stages = (224 * 1024 - nq * tile) / tile;
     x.vs = min(stages / 2, STAGES_MAX), x.ks = min(stages - x.vs, STAGES_MAX);
     const size_t smem = (size_t)(nq + x.ks + x.vs) * tile;
-    auto kern = long_tiles<D>;
+    auto kern = long_tiles<D, G>;
     static bool allowed[64];
     if (const int rc = b2_allow_smem(reinterpret_cast<const void*>(kern), allowed)) return rc;
-    cudaLaunchConfig_t cfg;
-    memset(&cfg, 0, sizeof cfg);
-    cfg.gridDim = dim3(a.ctas), cfg.blockDim = dim3(TW * 32), cfg.dynamicSmemBytes = smem, cfg.stream = s;
-    if (cudaLaunchKernelEx(&cfg, kern, tm[0], tm[1], tm[2], tm[3], x) != cudaSuccess) {
-        (void)cudaGetLastError();
-        return B2_ERR_CUDA;
-    }
-    return B2_OK;
+    return launch(kern, dim3(a.ctas), dim3(TW * 32), smem, s, tm[0], tm[1], tm[2], tm[3], x);
 }
 template <int D, int G>
 int launch_long(const LongArgs& a, cudaStream_t s) {
-    if (const int rc = launch_tiles<D>(a, s)) return rc;
-    if (const int rc = b2_launch(reinterpret_cast<const void*>(long_join<D, G>), dim3(a.T, a.Hk), dim3(JW * 32), 0, s, a)) return rc;
-    if (a.totals == nullptr) return B2_OK;
+    if (const int rc = launch_tiles<D, G>(a, s)) return rc;
+    // (blocks enough for a key a thread of the whole cache, or for the card)
+    const int wb = a.scores != nullptr ? min((a.cap + JT - 1) / JT, max(1, 8 * a.ctas / a.Hk)) : 0;
+    if (const int rc = launch(long_join<D, G>, dim3(a.T * a.Hq + wb * a.Hk), dim3(JT), 0, s, a, wb)) return rc;
+    if (a.totals == nullptr || a.scores != nullptr) return B2_OK;
     auto kern = long_weights<D, G>;
     static bool allowed[64];
     if (const int rc = b2_allow_smem(reinterpret_cast<const void*>(kern), allowed)) return rc;
-    return b2_launch(reinterpret_cast<const void*>(kern), dim3((a.cap + WK - 1) / WK, a.Hk), dim3(WK), (size_t)a.T * G * D * 2, s, a);
+    return launch(kern, dim3((a.cap + WK - 1) / WK, a.Hk), dim3(WK), (size_t)a.T * G * D * 2, s, a);
 }
 template <int D>
 int launch_long_g(const LongArgs& a, cudaStream_t s) {
@@ -933,7 +1044,15 @@ int check_cache(const void* q, const void* K, const void* V, const void* out, in
 }  // namespace
 
 extern "C" size_t btb_b200_attn_shared_workspace_bytes(int T, int Hq, int Hk, int D) {
-    return shape_ok(T, Hq, Hk, D) ? part_rows(T, Hq) * (D * 4 + 8) : 0;
+    return shape_ok(T, Hq, Hk, D) ? state_rows(T, Hq, Hk) * (D * 4 + 8) : 0;
+}
+
+// the states' place in a workspace; returns what lies behind it
+static float* take_states(LongArgs& a, void* workspace, int D) {
+    const size_t rows = state_rows(a.T, a.Hq, a.Hk);
+    a.part_o = static_cast<float*>(workspace), a.part_ml = reinterpret_cast<float2*>(a.part_o + rows * D);
+    a.unit_row = (long long)part_rows(a.T, a.Hq);
+    return reinterpret_cast<float*>(a.part_ml + rows);
 }
 
 extern "C" int btb_b200_attn_shared(const void* q, const void* K, const void* V, void* out, const void* rw, int T, int Hq,
@@ -945,13 +1064,15 @@ extern "C" int btb_b200_attn_shared(const void* q, const void* K, const void* V,
     a.q = static_cast<const bf16*>(q), a.K = static_cast<const bf16*>(K), a.V = static_cast<const bf16*>(V);
     a.out = static_cast<bf16*>(out), a.rw = static_cast<const int*>(rw), a.sinks = static_cast<const float*>(sinks);
     a.scale = scale, a.T = T, a.Hq = Hq, a.Hk = Hk, a.win = win, a.cap = cap, a.ctas = long_ctas(), a.hs = hs, a.rs = rs;
-    a.part_o = static_cast<float*>(workspace), a.part_ml = reinterpret_cast<float2*>(a.part_o + part_rows(T, Hq) * D);
+    (void)take_states(a, workspace, D);
     return D == 64 ? launch_long_g<64>(a, static_cast<cudaStream_t>(stream)) : launch_long_g<128>(a, static_cast<cudaStream_t>(stream));
 }
 
 extern "C" size_t btb_b200_attn_scored_workspace_bytes(int T, int Hq, int Hk, int D, int cap) {
     if (!shape_ok(T, Hq, Hk, D) || cap <= 0) return 0;
-    return part_rows(T, Hq) * (D * 4 + 8) + (size_t)T * Hq * 33 * 4;
+    size_t n = state_rows(T, Hq, Hk) * (D * 4 + 8) + (size_t)T * Hq * 33 * 4;
+    if (keeps_scores(T, Hq, Hk)) n = ((n + 15) & ~(size_t)15) + (size_t)T * Hq * score_stride(cap) * 4;
+    return n;
 }
 
 extern "C" int btb_b200_attn_scored(const void* q, const void* K, const void* V, void* out, const void* n0p, const void* par,
@@ -966,7 +1087,10 @@ extern "C" int btb_b200_attn_scored(const void* q, const void* K, const void* V,
     a.tbl = static_cast<const int*>(tbl), a.sinks = static_cast<const float*>(sinks);
     a.totals = static_cast<float*>(totals), a.ts = ts;
     a.scale = scale, a.T = T, a.Hq = Hq, a.Hk = Hk, a.cap = cap, a.ctas = long_ctas(), a.hs = hs, a.rs = rs;
-    a.part_o = static_cast<float*>(workspace), a.part_ml = reinterpret_cast<float2*>(a.part_o + part_rows(T, Hq) * D);
-    a.lse = reinterpret_cast<float*>(a.part_ml + part_rows(T, Hq)), a.own = a.lse + (size_t)T * Hq;
+    a.lse = take_states(a, workspace, D), a.own = a.lse + (size_t)T * Hq;
+    if (keeps_scores(T, Hq, Hk)) {
+        const uintptr_t past = reinterpret_cast<uintptr_t>(a.own + (size_t)T * Hq * 32);
+        a.scores = reinterpret_cast<float*>((past + 15) & ~(uintptr_t)15), a.score_n = score_stride(cap);
+    }
     return D == 64 ? launch_long_g<64>(a, static_cast<cudaStream_t>(stream)) : launch_long_g<128>(a, static_cast<cudaStream_t>(stream));
 }

@@ -15,7 +15,8 @@ struct B2Tuning {
     int ctas_per_sm;  // GEMV CTAs an SM (the grid is persistent)
     int evict_first;  // weight copies carry an L2 evict-first hint
     int pdl;          // programmatic stream serialization: bit 0 the GEMV launches, bit 1 the step's small kernels,
-                      // bit 2 the MoE block's kernels (router, picked experts, activation, sum)
+                      // bit 2 the MoE block's kernels (router, picked experts, activation, sum), bit 3 the long-cache
+                      // attention's
     int warps;        // warps a GEMV CTA for passes of one or two rows: 8 or 16
     int solo;         // under PDL a GEMV CTA claims an SM's shared memory for itself
     int moe_stream;   // the picked experts' matvecs through the streaming kernel (0: the plain 16-lane kernel)

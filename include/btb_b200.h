@@ -33,7 +33,8 @@ extern "C" {
 int btb_b200_version(void);
 int btb_b200_sm_count(void);
 /* tunables: "ring_bytes", "seg_bytes", "x_smem_max", "ctas_per_sm", "evict_first", "pdl" (a mask: 1 the GEMV launches,
- * 2 the step's small kernels, 4 the MoE block's kernels start under programmatic dependent launch; default 5), "warps",
+ * 2 the step's small kernels, 4 the MoE block's kernels, 8 the long-cache attention's start under programmatic dependent
+ * launch; default 13), "warps",
  * "balance", "solo", "moe_stream" (host string) */
 int btb_b200_set_tuning(const char* key, int value);
 /* reads the device status word into *code (host pointer) and clears it; synchronises the default stream's copy */
