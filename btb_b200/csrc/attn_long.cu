@@ -39,12 +39,12 @@ struct LongArgs {
 
 // ---- the pass's work, from what stands on the card ------------------------------------------------------------------
 // The prefixes: per kv head an item for each prefix that rows share, its queries all of those rows', its keys cut into
-// tiles of 128. The tiles of all heads in one line are cut evenly over the CTAs; a CTA's stretch of an item is a part, whose
+// tiles of 64. The tiles of all heads in one line are cut evenly over the CTAs; a CTA's stretch of an item is a part, whose
 // state (maximum, sum, output row) the joining kernel folds with the others'. Part (CTA c, item i) keeps its rows at
 // c * T G + the rows of all items before i, which no two parts share.
 // A row's own keys (its steps in the rows layout, its path in a chain or tree pass) are no one else's: units of up to
 // `chunk` keys of one (row, kv head), a warp each, beside the tiles. A one-row pass's own key joins its prefix.
-constexpr int KT = 128;        // keys a tile
+constexpr int KT = 64;         // keys a tile
 constexpr int CTAS_MAX = 160;  // CTAs of the tile kernel at most
 constexpr int OWN_WARPS = 2;   // warps of a CTA that take units (two more would leave all of them 128 registers)
 
@@ -52,6 +52,7 @@ struct Plan {
     int mask[32];                             // item of lane l's prefix: its rows (0: no item)
     int p_start[32], p_count[32];             // ... its first key (cache row, or logical row of a chain or tree pass) and keys
     int p_tiles[32], p_tile0[32], p_row0[32]; // ... tiles, tiles and partial rows before it (within a kv head)
+    int order[32];                            // ... its rows, from p_row0 / G on
     int lead[32];                             // row t's prefix item, -1: padding or refused
     int own[32], own_n[32], unit0[32];        // its own keys: the first's cache row (rows layout), how many; units before it
     int W, tiles, rows, units, chunk, n0;     // ... and the kv head's tiles, partial rows and units
@@ -129,37 +130,45 @@ __device__ __forceinline__ void make_plan(const LongArgs& A, int G, Plan& P, boo
     const int unit0 = warp_excl(own_n > 0 ? (own_n + chunk - 1) / chunk : 0, t, units);
     P.mask[t] = mask, P.p_start[t] = start, P.p_count[t] = count, P.p_tiles[t] = p_tiles, P.p_tile0[t] = p_tile0, P.p_row0[t] = p_row0;
     P.lead[t] = lead, P.own[t] = own, P.own_n[t] = own_n, P.unit0[t] = unit0;
+    const int src = lead < 0 ? 0 : lead;
+    const int its = __shfl_sync(0xffffffffu, mask, src), before = __shfl_sync(0xffffffffu, p_row0, src), some = __shfl_sync(0xffffffffu, p_tiles, src);
+    if (lead >= 0 && some > 0) P.order[before / G + __popc(its & ((1u << t) - 1u))] = t;
     if (t == 0) P.W = W, P.tiles = pt, P.rows = pr, P.units = units, P.chunk = chunk, P.n0 = n0;
     __syncwarp();
 }
 
-// where CTA c's stretch of `tiles` tiles begins; only as many of the `ctas` CTAs have one as there are tiles, so that no
-// stretch between two others is empty
-__device__ __forceinline__ long long first_tile(long long tiles, int c, int ctas) {
-    const long long n = min((long long)ctas, tiles);
-    return c >= n ? tiles : tiles * c / n;
-}
+// the even cut of `tiles` tiles over the CTAs; only as many of them have any as there are tiles, so that no stretch between
+// two others is empty
+struct Cut {
+    int per, more;  // the first `more` CTAs have per + 1 tiles
+    __device__ __forceinline__ Cut(int tiles, int ctas) : per(tiles / ctas), more(tiles - tiles / ctas * ctas) {}
+    __device__ __forceinline__ int first(int c) const { return c * per + min(c, more); }
+    __device__ __forceinline__ int cta_of(int tile) const {
+        const int big = more * (per + 1);
+        return tile < big ? tile / (per + 1) : more + (tile - big) / per;
+    }
+};
 
 // a CTA's stretch of one item
 struct Part {
-    int head, mask, start, keys, tiles, rows;  // `keys`: of these tiles (the last may be partly filled)
-    long long row0;                            // its first partial row
-    long long end;                             // the first tile past it
+    int head, start, keys, tiles, rows, order;  // `keys`: of these tiles (the last may be partly filled)
+    int end;                                    // the first tile past it
+    long long row0;                             // its first partial row
 };
 // the part that begins at tile `at` of a CTA whose stretch ends at `stop` (every lane of a warp asks alike)
-__device__ __forceinline__ Part part_at(const Plan& P, const LongArgs& A, int G, long long at, long long stop, int cta) {
+__device__ __noinline__ Part part_at(const Plan& P, int span, int G, int at, int stop, int cta) {
     const int lane = threadIdx.x & 31;
     Part p;
-    p.head = (int)(at / P.tiles);
-    const int in = (int)(at - (long long)p.head * P.tiles);
+    p.head = at / P.tiles;
+    const int in = at - p.head * P.tiles;
     const int l = __ffs(__ballot_sync(0xffffffffu, in >= P.p_tile0[lane] && in < P.p_tile0[lane] + P.p_tiles[lane])) - 1;
     const int skip = in - P.p_tile0[l];
-    p.tiles = (int)min((long long)(P.p_tiles[l] - skip), stop - at);
-    p.mask = P.mask[l];
+    p.tiles = min(P.p_tiles[l] - skip, stop - at);
     p.start = P.p_start[l] + skip * KT;
     p.keys = min(p.tiles * KT, P.p_count[l] - skip * KT);
-    p.rows = __popc(p.mask) * G;
-    p.row0 = (long long)cta * A.T * G + (long long)p.head * P.rows + P.p_row0[l];
+    p.rows = __popc(P.mask[l]) * G;
+    p.order = P.p_row0[l] / G;
+    p.row0 = (long long)cta * span + (long long)p.head * P.rows + P.p_row0[l];
     p.end = at + p.tiles;
     return p;
 }
@@ -168,8 +177,9 @@ __device__ __forceinline__ Part part_at(const Plan& P, const LongArgs& A, int G,
 // S = Q K^T and O += P V with tcgen05.mma: up to 128 of an item's query rows (row-of-the-pass major, then the kv head's query
 // heads) are the MMA's M, so a shared key is read once for all of them. Two warpgroups turn scores into weights, a thread a
 // query row, on alternate key tiles with an output accumulator each (items of up to 128 rows; the two are folded at the
-// part's end) or on the two halves of an item's up to 256 rows. Scores, weights (over their scores) and outputs live in
-// tensor memory: S0 S1 O0 O1, 128 columns each.
+// part's end) or on the two halves of an item's up to 256 rows. Tensor memory, 512 columns: two score tiles of 64 columns a
+// warpgroup, so that the next one is there when a warpgroup comes from the last, then the two outputs; weights (bf16) lie over
+// their scores.
 __device__ __forceinline__ uint64_t desc_sw128(uint32_t saddr, uint32_t lbo) {
     return (uint64_t)((saddr & 0x3FFFFu) >> 4) | ((uint64_t)(lbo >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) |
            ((uint64_t)2 << 61);
@@ -247,17 +257,17 @@ __device__ __forceinline__ void tma_rows4(uint32_t dst, const CUtensorMap* tm, i
 }
 
 constexpr int TW = 10 + OWN_WARPS;  // warps: two warpgroups for the weights, the loads' warp, the MMAs' warp, the units' warps
-constexpr int STAGES_MAX = 6;   // stages of a ring
+constexpr int STAGES_MAX = 12;      // stages of a ring
 
 struct alignas(8) TileSync {
     uint64_t kfull[STAGES_MAX], kempty[STAGES_MAX], vfull[STAGES_MAX], vempty[STAGES_MAX];
-    uint64_t sfull[2];   // a warpgroup's scores are there
-    uint64_t pready[2];  // ... its weights are
-    uint64_t odone[2];   // ... its last product of a part is added
-    uint64_t qfull;      // the part's queries are in shared memory
-    uint64_t stats;      // the second warpgroup's maxima and sums are in shared memory
-    uint64_t next;       // both warpgroups are through with the part
-    uint64_t drain;      // every MMA has run
+    uint64_t sfull[2][2];   // a warpgroup's scores are there, a buffer each
+    uint64_t pready[2][2];  // ... its weights are
+    uint64_t pv[2][2];      // ... their product with the values is added
+    uint64_t qfull;         // the part's queries are in shared memory
+    uint64_t stats;         // the second warpgroup's maxima and sums are in shared memory
+    uint64_t next;          // both warpgroups are through with the part
+    uint64_t drain;         // every MMA has run
     uint32_t tmem;
     int fail;
 };
@@ -265,7 +275,7 @@ struct alignas(8) TileSync {
 struct TileArgs {
     LongArgs a;
     int row_mul, col_mul;  // a kv head's rows begin at head * row_mul, its columns at head * col_mul
-    int ks, vs;            // stages of the rings
+    int stages;            // of either ring
 };
 
 // a warp's bounded wait that also ends once any other role has given up; its lanes get one answer
@@ -357,18 +367,16 @@ __device__ __forceinline__ void own_units(const LongArgs& A, const Plan& P, int 
 #pragma unroll 1
             for (int k0 = 0; k0 < 32; k0 += VB) {
                 if (k0 >= n - j0) break;
-                unsigned short v[VB][E];
+                uint32_t v[VB][E / 2];
 #pragma unroll
                 for (int k = 0; k < VB; ++k) {  // (a key outside has weight 0 over zeros)
                     const int r = __shfl_sync(0xffffffffu, row, k0 + k);
                     const bf16* vr = Vg + (size_t)max(r, 0) * A.rs + lane * E;
                     if (E == 4) {
                         const uint2 x = r >= 0 ? __ldg(reinterpret_cast<const uint2*>(vr)) : make_uint2(0u, 0u);
-                        split_bf16(x.x, v[k][0], v[k][1]);
-                        split_bf16(x.y, v[k][E - 2], v[k][E - 1]);
+                        v[k][0] = x.x, v[k][E / 2 - 1] = x.y;
                     } else {
-                        const uint32_t x = r >= 0 ? __ldg(reinterpret_cast<const uint32_t*>(vr)) : 0u;
-                        split_bf16(x, v[k][0], v[k][E - 1]);
+                        v[k][0] = r >= 0 ? __ldg(reinterpret_cast<const uint32_t*>(vr)) : 0u;
                     }
                 }
 #pragma unroll
@@ -377,7 +385,10 @@ __device__ __forceinline__ void own_units(const LongArgs& A, const Plan& P, int 
                     for (int hh = 0; hh < G; ++hh) {
                         const float p = __shfl_sync(0xffffffffu, s[hh], k0 + k);
 #pragma unroll
-                        for (int e = 0; e < E; ++e) o[hh][e] = fmaf(p, __uint_as_float((uint32_t)v[k][e] << 16), o[hh][e]);
+                        for (int e = 0; e < E; e += 2) {
+                            o[hh][e] = fmaf(p, bf_lo(v[k][e / 2]), o[hh][e]);
+                            o[hh][e + 1] = fmaf(p, bf_hi(v[k][e / 2]), o[hh][e + 1]);
+                        }
                     }
             }
         }
@@ -396,25 +407,26 @@ template <int D, int G>
 __global__ void __launch_bounds__(TW * 32, 1)
     long_tiles(const __grid_constant__ CUtensorMap kbox, const __grid_constant__ CUtensorMap krows,
                const __grid_constant__ CUtensorMap vbox, const __grid_constant__ CUtensorMap vrows, const TileArgs X) {
-    constexpr int TILE = KT * D * 2;    // bytes of a tile of keys, values or queries: D / 64 blocks of 128 rows x 128 bytes
-    constexpr int HALF = KT * 128;
+    constexpr int TILE = KT * D * 2, QTILE = 128 * D * 2;  // bytes of a tile of keys or values, and of queries:
+    constexpr int HALF = KT * 128, QHALF = 128 * 128;      // D / 64 blocks of rows of 128 bytes
     const LongArgs& A = X.a;
-    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    extern __shared__ __align__(1024) uint8_t smem[];
     __shared__ TileSync sy;
     __shared__ Plan plan;
     __shared__ float s_m[128], s_l[128];
-    uint8_t* smem = smem_raw;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int nq = A.T * G > 128 ? 2 : 1;
-    const uint32_t sq = smem_u32(smem), sk = sq + nq * TILE, sv = sk + X.ks * TILE;
+    const uint32_t sq = smem_u32(smem), sk = sq + nq * QTILE, sv = sk + X.stages * TILE;
 
     if (threadIdx.x == 32) {
-        for (int s = 0; s < STAGES_MAX; ++s) {
+        for (int s = 0; s < X.stages; ++s) {
             mbar_init(smem_u32(&sy.kfull[s]), 1), mbar_init(smem_u32(&sy.kempty[s]), 1);
             mbar_init(smem_u32(&sy.vfull[s]), 1), mbar_init(smem_u32(&sy.vempty[s]), 1);
         }
-        for (int w = 0; w < 2; ++w)
-            mbar_init(smem_u32(&sy.sfull[w]), 1), mbar_init(smem_u32(&sy.pready[w]), 4), mbar_init(smem_u32(&sy.odone[w]), 1);
+        for (int w = 0; w < 2; ++w) {
+            for (int b = 0; b < 2; ++b)
+                mbar_init(smem_u32(&sy.sfull[w][b]), 1), mbar_init(smem_u32(&sy.pready[w][b]), 4), mbar_init(smem_u32(&sy.pv[w][b]), 1);
+        }
         mbar_init(smem_u32(&sy.qfull), 8), mbar_init(smem_u32(&sy.stats), 4), mbar_init(smem_u32(&sy.next), 8);
         mbar_init(smem_u32(&sy.drain), 1);
         sy.fail = 0;
@@ -425,8 +437,8 @@ __global__ void __launch_bounds__(TW * 32, 1)
     pdl_launch_dependents();
     if (warp == 0) make_plan(A, G, plan, blockIdx.x == 0);
     __syncthreads();
-    const long long all = (long long)plan.tiles * A.Hk;
-    const long long begin = first_tile(all, blockIdx.x, gridDim.x), stop = first_tile(all, blockIdx.x + 1, gridDim.x);
+    const Cut cut(plan.tiles * A.Hk, gridDim.x);
+    const int begin = cut.first(blockIdx.x), stop = cut.first(blockIdx.x + 1);
     if (begin >= stop) {  // no tiles for this CTA: nothing allocated yet
         if (warp >= 10) own_units<D, G>(A, plan, (warp - 10) * gridDim.x + blockIdx.x, OWN_WARPS * gridDim.x);
         return;
@@ -450,24 +462,28 @@ __global__ void __launch_bounds__(TW * 32, 1)
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
         const uint32_t ts = tmem + lanes + wg * 128, to = tmem + lanes + 256 + wg * 128;
         const float scale2 = fabsf(__fmul_rn(A.scale, LOG2E));  // (a negative scale's sign is the queries')
-        uint32_t sph = 0, oph = 0, stph = 0, nph = 0;
+        uint32_t count = 0;                                     // this warpgroup's tiles so far
+        uint32_t stph = 0, nph = 0;
         bool ok = true;
-        for (long long at = begin; at < stop && ok;) {
-            const Part p = part_at(plan, A, G, at, stop, blockIdx.x);
+        for (int at = begin; at < stop && ok;) {
+            const Part p = part_at(plan, A.T * G, G, at, stop, blockIdx.x);
             at = p.end;
             const bool two = p.rows > 128;
             {   // the part's queries into shared memory as the MMA reads them: 16-byte piece c of row r at c ^ (r & 7)
                 const uint32_t flip = A.scale < 0.f ? 0x80008000u : 0u;
+#pragma unroll 1
                 for (int rt = 0; rt < (two ? 2 : 1); ++rt) {
                     const int r = rt * 128 + row;
-                    const int t = r < p.rows ? (int)__fns(p.mask, 0, r / G + 1) : 0;
+                    const int t = r < p.rows ? plan.order[p.order + r / G] : 0;
                     const uint4* src = reinterpret_cast<const uint4*>(A.q + ((size_t)t * A.Hq + p.head * G + r % G) * D) + wg * (D / 16);
+                    uint4 v[D / 16];
+#pragma unroll
+                    for (int c = 0; c < D / 16; ++c) v[c] = r < p.rows ? src[c] : make_uint4(0u, 0u, 0u, 0u);
 #pragma unroll
                     for (int c = 0; c < D / 16; ++c) {
-                        uint4 v = r < p.rows ? src[c] : make_uint4(0u, 0u, 0u, 0u);
-                        v.x ^= flip, v.y ^= flip, v.z ^= flip, v.w ^= flip;
+                        v[c].x ^= flip, v[c].y ^= flip, v[c].z ^= flip, v[c].w ^= flip;
                         const int piece = wg * (D / 16) + c;
-                        *reinterpret_cast<uint4*>(smem + rt * TILE + (piece >> 3) * HALF + row * 128 + (((piece & 7) ^ (row & 7)) << 4)) = v;
+                        *reinterpret_cast<uint4*>(smem + rt * QTILE + (piece >> 3) * QHALF + row * 128 + (((piece & 7) ^ (row & 7)) << 4)) = v[c];
                     }
                 }
                 fence_proxy_async();
@@ -477,34 +493,37 @@ __global__ void __launch_bounds__(TW * 32, 1)
             const int mine = two ? p.tiles : (p.tiles + 1 - wg) >> 1;  // this warpgroup's tiles
             const int valid = two ? p.rows - wg * 128 : p.rows;        // ... and query rows
             const bool idle = (warp & 3) * 32 >= valid;
+            float* keep = nullptr;  // where this row's scores go
+            if (A.scores != nullptr && row < valid)
+                keep = A.scores + ((size_t)p.head * p.rows + row) * A.score_n + p.start + wg * KT;
             float m = NEG_INF, l = 0.f;
-            for (int i = 0; i < mine; ++i) {
-                if (!(ok = wait_or_fail(&sy.sfull[wg], sph, sy))) break;
-                sph ^= 1;
+#pragma unroll 1
+            for (int i = 0; i < mine; ++i, ++count) {
+                const int b = count & 1;
+                if (!(ok = wait_or_fail(&sy.sfull[wg][b], (count >> 1) & 1, sy))) break;
                 tm_after();
                 if (!idle) {
                     const int left = p.keys - (two ? i : 2 * i + wg) * KT;  // keys from this tile's first on
-                    // (the scores are read twice, for the maximum and for the weights: held over, they would spill)
                     uint32_t s[2][32];
-                    float mx[4] = {NEG_INF, NEG_INF, NEG_INF, NEG_INF};
-                    tm_ld32(ts, s[0]);
+                    tm_ld32(ts + b * KT, s[0]);
+                    tm_ld32(ts + b * KT + 32, s[1]);
+                    tm_wait_ld(s[0]);
+                    tm_wait_ld(s[1]);
+                    if (left < KT) {
 #pragma unroll
-                    for (int c0 = 0; c0 < KT; c0 += 32) {
-                        uint32_t(&v)[32] = s[(c0 >> 5) & 1];
-                        tm_wait_ld(v);
-                        tm_ld32(ts + (c0 + 32 < KT ? c0 + 32 : 0), s[((c0 >> 5) & 1) ^ 1]);  // (last: the first again)
-                        if (left < c0 + 32) {
-#pragma unroll
-                            for (int c = 0; c < 32; ++c) v[c] = c0 + c < left ? v[c] : 0xff800000u;
-                        }
-#pragma unroll
-                        for (int c = 0; c < 32; ++c) mx[c & 3] = fmaxf(mx[c & 3], __uint_as_float(v[c]));
+                        for (int c = 0; c < KT; ++c) s[c >> 5][c & 31] = c < left ? s[c >> 5][c & 31] : 0xff800000u;
                     }
+                    float mx[4] = {NEG_INF, NEG_INF, NEG_INF, NEG_INF};
+#pragma unroll
+                    for (int c = 0; c < KT; ++c) mx[c & 3] = fmaxf(mx[c & 3], __uint_as_float(s[c >> 5][c & 31]));
                     const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale2;
                     // The weights are taken relative to a reference that follows the maximum only when that has risen by more
                     // than 8 (a factor of 256, which sums and bf16 weights hold without loss): most tiles leave the output alone.
                     const float ref = i == 0 ? top : (top > m + 8.f ? top : m);
                     if (i > 0 && __any_sync(0xffffffffu, ref != m)) {
+                        // (the product before must be in: the one before that is, these scores were asked for after it)
+                        if (!(ok = wait_or_fail(&sy.pv[wg][b ^ 1], ((count - 1) >> 1) & 1, sy))) break;
+                        tm_after();
                         const float f = m == NEG_INF ? 0.f : ex2(m - ref);
                         l *= f;
 #pragma unroll 1
@@ -519,51 +538,39 @@ __global__ void __launch_bounds__(TW * 32, 1)
                     }
                     m = ref;
                     const float sub = m == NEG_INF ? 0.f : m;
+                    if (keep != nullptr) {
+                        float* to_row = keep + (size_t)i * (two ? KT : 2 * KT);
+#pragma unroll
+                        for (int c = 0; c < KT; c += 4)
+                            *reinterpret_cast<float4*>(to_row + c) =
+                                make_float4(__uint_as_float(s[c >> 5][c & 31]) * scale2, __uint_as_float(s[c >> 5][(c & 31) + 1]) * scale2,
+                                            __uint_as_float(s[c >> 5][(c & 31) + 2]) * scale2, __uint_as_float(s[c >> 5][(c & 31) + 3]) * scale2);
+                    }
                     float sum[4] = {0.f, 0.f, 0.f, 0.f};
-                    float* keep = nullptr;  // where this row's scores go
-                    if (A.scores != nullptr && row < valid)
-                        keep = A.scores + ((size_t)p.head * p.rows + row) * A.score_n + p.start + (size_t)(two ? i : 2 * i + wg) * KT;
 #pragma unroll
-                    for (int c0 = 0; c0 < KT; c0 += 32) {
-                        uint32_t(&v)[32] = s[(c0 >> 5) & 1];
+                    for (int h = 0; h < 2; ++h) {
                         uint32_t w[16];
-                        tm_wait_ld(v);
-                        if (c0 + 32 < KT) tm_ld32(ts + c0 + 32, s[((c0 >> 5) & 1) ^ 1]);
-                        if (left < c0 + 32) {
-#pragma unroll
-                            for (int c = 0; c < 32; ++c) v[c] = c0 + c < left ? v[c] : 0xff800000u;
-                        }
 #pragma unroll
                         for (int c = 0; c < 16; ++c) {
-                            const float a = ex2(fmaf(__uint_as_float(v[2 * c]), scale2, -sub));
-                            const float b = ex2(fmaf(__uint_as_float(v[2 * c + 1]), scale2, -sub));
-                            sum[(2 * c) & 3] += a, sum[(2 * c + 1) & 3] += b;
-                            asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w[c]) : "f"(b), "f"(a));
+                            const float x = ex2(fmaf(__uint_as_float(s[h][2 * c]), scale2, -sub));
+                            const float y = ex2(fmaf(__uint_as_float(s[h][2 * c + 1]), scale2, -sub));
+                            sum[(2 * c) & 3] += x, sum[(2 * c + 1) & 3] += y;
+                            asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w[c]) : "f"(y), "f"(x));
                         }
-                        tm_st16(ts + c0 / 2, w);
-                        if (keep != nullptr) {
-#pragma unroll
-                            for (int c = 0; c < 32; c += 4)
-                                *reinterpret_cast<float4*>(keep + c0 + c) =
-                                    make_float4(__uint_as_float(v[c]) * scale2, __uint_as_float(v[c + 1]) * scale2,
-                                                __uint_as_float(v[c + 2]) * scale2, __uint_as_float(v[c + 3]) * scale2);
-                        }
+                        tm_st16(ts + b * KT + h * 16, w);
                     }
                     l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
                     tm_wait_st();
                 }
                 tm_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(smem_u32(&sy.pready[wg]));
+                if (lane == 0) mbar_arrive(smem_u32(&sy.pready[wg][b]));
             }
             // ---- the part's state ----------------------------------------------------------------------------------------
-            if (ok && mine > 0) {
-                ok = wait_or_fail(&sy.odone[wg], oph, sy);
-                oph ^= 1;
-                tm_after();
-            }
+            if (ok && mine > 0) ok = wait_or_fail(&sy.pv[wg][(count - 1) & 1], ((count - 1) >> 1) & 1, sy);
+            tm_after();
             if (!two && wg == 1) {
-                s_m[row] = mine > 0 ? m : NEG_INF, s_l[row] = l;
+                s_m[row] = m, s_l[row] = l;
                 tm_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(smem_u32(&sy.stats));
@@ -574,36 +581,39 @@ __global__ void __launch_bounds__(TW * 32, 1)
             }
             if (!two) stph ^= 1;
             if (ok && !idle && (two || wg == 0)) {
-                const int r = wg * 128 + row;  // (two: the warpgroup's half; else the first's)
                 const bool other = !two && p.tiles > 1;
                 float f0 = 1.f, f1 = 0.f, M = m, L = l;
-                if (other) {
-                    fold_ml(M, L, s_m[row], s_l[row], f0, f1);
-                }
-                const size_t at_row = (size_t)(p.row0 + r);
+                if (other) fold_ml(M, L, s_m[row], s_l[row], f0, f1);
+                const size_t row0 = (size_t)(p.row0 + warp * 32);  // the warp's first row (two: the second warpgroup's from 128 on)
+                const int rows = min(32, valid - (warp & 3) * 32);
+                // by way of the queries' place (all scores are made), so that a row's 32 columns are stored by eight lanes side by
+                // side: row r, piece c of 16 bytes at c ^ (r & 7)
+                uint8_t* mid = smem + warp * 4096;
 #pragma unroll 1
                 for (int c = 0; c < D; c += 32) {
-                    uint32_t o[32], o2[32];
+                    uint32_t o[32];
                     tm_ld32(to + c, o);
+                    tm_wait_ld(o);
                     if (other) {
+                        uint32_t o2[32];
                         tm_ld32(to + 128 + c, o2);
                         tm_wait_ld(o2);
-                    }
-                    tm_wait_ld(o);
-                    if (row < valid) {
 #pragma unroll
-                        for (int k = 0; k < 32; k += 4) {
-                            float4 v = make_float4(__uint_as_float(o[k]), __uint_as_float(o[k + 1]), __uint_as_float(o[k + 2]),
-                                                   __uint_as_float(o[k + 3]));
-                            if (other) {
-                                v.x = fold_e(v.x, __uint_as_float(o2[k]), f0, f1), v.y = fold_e(v.y, __uint_as_float(o2[k + 1]), f0, f1);
-                                v.z = fold_e(v.z, __uint_as_float(o2[k + 2]), f0, f1), v.w = fold_e(v.w, __uint_as_float(o2[k + 3]), f0, f1);
-                            }
-                            *reinterpret_cast<float4*>(A.part_o + at_row * D + c + k) = v;
-                        }
+                        for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(fold_e(__uint_as_float(o[k]), __uint_as_float(o2[k]), f0, f1));
                     }
+#pragma unroll
+                    for (int k = 0; k < 8; ++k)
+                        *reinterpret_cast<uint4*>(mid + lane * 128 + ((k ^ (lane & 7)) << 4)) = make_uint4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
+                    __syncwarp();
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) {
+                        const int r = k * 4 + (lane >> 3), piece = lane & 7;
+                        const uint4 v = *reinterpret_cast<const uint4*>(mid + r * 128 + ((piece ^ (r & 7)) << 4));
+                        if (r < rows) *reinterpret_cast<uint4*>(A.part_o + (row0 + r) * D + c + piece * 4) = v;
+                    }
+                    __syncwarp();
                 }
-                if (row < valid) A.part_ml[at_row] = make_float2(M, L);
+                if (lane < rows) A.part_ml[row0 + lane] = make_float2(M, L);
             }
             tm_before();
             __syncwarp();
@@ -614,28 +624,25 @@ __global__ void __launch_bounds__(TW * 32, 1)
         }
     } else if (warp == 8) {
         // ---- the loads --------------------------------------------------------------------------------------------------------
-        int ks = 0, vs = 0;
-        uint32_t kph = 0, vph = 0;
-        long long kn = 0, vn = 0;  // tiles begun
+        int st = 0, asked[2] = {0, 0};  // copies of keys and of values begun
+        uint32_t ph = 1;                // (the first round finds the stages empty)
         bool ok = true;
-        for (long long at = begin; at < stop && ok;) {
-            const Part p = part_at(plan, A, G, at, stop, blockIdx.x);
+        for (int at = begin; at < stop && ok;) {
+            const Part p = part_at(plan, A.T * G, G, at, stop, blockIdx.x);
             at = p.end;
             const int x = p.head * X.col_mul, y0 = p.head * X.row_mul;
-            const bool mapped = A.tbl != nullptr;
+#pragma unroll 1
             for (int i = 0; i < p.tiles && ok; ++i) {
                 const int keys = min(KT, p.keys - i * KT);
-                const bool box = keys == KT && !mapped;
+                const bool box = keys == KT && A.tbl == nullptr;
                 int y[4];
-                if (box) {
-                    y[0] = y0 + p.start + i * KT;
-                } else {
-                    // rows 4 lane .. 4 lane + 3 of the tile; past its keys the last one again (its weight there is 0: the
-                    // values multiplied by it must be ones that the rows see)
+                if (!box) {
+                    // sixteen lanes four rows each (and each half of them 64 columns); past the tile's keys the last one again
+                    // (its weight there is 0: the values multiplied by it must be ones that the rows see)
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {
-                        const int j = p.start + i * KT + min(lane * 4 + k, keys - 1);
-                        int r = mapped ? A.tbl[j] : j;
+                        const int j = p.start + i * KT + min((lane & 15) * 4 + k, keys - 1);
+                        int r = A.tbl != nullptr ? A.tbl[j] : j;
                         if (r < 0 || r >= A.cap) {
                             b2_fail(B2_ERR_DOMAIN);
                             r = 0;
@@ -643,91 +650,82 @@ __global__ void __launch_bounds__(TW * 32, 1)
                         y[k] = y0 + r;
                     }
                 }
-                for (int kv = 0; kv < 2 && ok; ++kv) {
-                    uint64_t* full = kv == 0 ? &sy.kfull[ks] : &sy.vfull[vs];
-                    uint64_t* empty = kv == 0 ? &sy.kempty[ks] : &sy.vempty[vs];
-                    const bool used = kv == 0 ? kn >= X.ks : vn >= X.vs;
-                    if (used && !(ok = wait_or_fail(empty, (kv == 0 ? kph : vph) ^ 1, sy))) break;
-                    const uint32_t bar = smem_u32(full), dst = kv == 0 ? sk + ks * TILE : sv + vs * TILE;
+#pragma unroll
+                for (int kv = 0; kv < 2; ++kv) {
+                    if (asked[kv] >= X.stages && !(ok = wait_or_fail(kv == 0 ? &sy.kempty[st] : &sy.vempty[st], ph, sy))) break;
+                    const uint32_t bar = smem_u32(kv == 0 ? &sy.kfull[st] : &sy.vfull[st]), dst = (kv == 0 ? sk : sv) + st * TILE;
                     if (lane == 0) mbar_expect_tx(bar, TILE);
                     __syncwarp();
                     if (box) {
-                        if (lane == 0)
-                            for (int c = 0; c < D / 64; ++c) tma_box(dst + c * HALF, kv == 0 ? &kbox : &vbox, x + c * 64, y[0], bar);
-                    } else {
-                        for (int c = 0; c < D / 64; ++c) tma_rows4(dst + c * HALF + lane * 512, kv == 0 ? &krows : &vrows, x + c * 64, y, bar);
+                        if (lane < D / 64) tma_box(dst + lane * HALF, kv == 0 ? &kbox : &vbox, x + lane * 64, y0 + p.start + i * KT, bar);
+                    } else if (lane < D / 4) {
+                        tma_rows4(dst + (lane >> 4) * HALF + (lane & 15) * 512, kv == 0 ? &krows : &vrows, x + (lane >> 4) * 64, y, bar);
                     }
-                    if (kv == 0) {
-                        ++kn;
-                        if (++ks == X.ks) ks = 0, kph ^= 1;
-                    } else {
-                        ++vn;
-                        if (++vs == X.vs) vs = 0, vph ^= 1;
-                    }
+                    ++asked[kv];
                 }
+                if (++st == X.stages) st = 0, ph ^= 1;
             }
         }
         // its copies have landed before the CTA ends (they have, unless some role gave up)
-        for (int s = 0; s < X.ks; ++s) {
-            const long long uses = kn / X.ks + (s < kn % X.ks ? 1 : 0);
-            if (uses > 0) (void)mbar_wait_bounded(smem_u32(&sy.kfull[s]), (uint32_t)(uses - 1) & 1);
-        }
-        for (int s = 0; s < X.vs; ++s) {
-            const long long uses = vn / X.vs + (s < vn % X.vs ? 1 : 0);
-            if (uses > 0) (void)mbar_wait_bounded(smem_u32(&sy.vfull[s]), (uint32_t)(uses - 1) & 1);
-        }
+        for (int s = 0; s < X.stages; ++s)
+#pragma unroll
+            for (int kv = 0; kv < 2; ++kv) {
+                const int uses = (asked[kv] + X.stages - 1 - s) / X.stages;
+                if (uses > 0) (void)mbar_wait_bounded(smem_u32(kv == 0 ? &sy.kfull[s] : &sy.vfull[s]), (uint32_t)(uses - 1) & 1);
+            }
     } else if (warp >= 10) {
         own_units<D, G>(A, plan, (warp - 10) * gridDim.x + blockIdx.x, OWN_WARPS * gridDim.x);
     } else {
         // ---- the MMAs -----------------------------------------------------------------------------------------------------------
-        // D f32, A and B bf16; S: both K-major, N = 128 keys; O: the values' dims are B's N and lie contiguous, N = D
+        // D f32, A and B bf16; S: both K-major, N = 64 keys; O: the values' dims are B's N and lie contiguous, N = D
         constexpr uint32_t base_desc = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(128 >> 4) << 24);
         constexpr uint32_t desc_s = base_desc | ((uint32_t)(KT >> 3) << 17), desc_o = base_desc | (1u << 16) | ((uint32_t)(D >> 3) << 17);
+        const uint64_t q0 = desc_sw128(sq, 0), k0 = desc_sw128(sk, 0), v0 = desc_sw128(sv, HALF);
         int ks = 0, vs = 0;
-        uint32_t kph = 0, vph = 0, pph[2] = {0, 0}, qph = 0;
+        uint32_t kph = 0, vph = 0, qph = 0, scount[2] = {0, 0}, pcount[2] = {0, 0};
         bool ok = true;
-        for (long long at = begin; at < stop && ok;) {
-            const Part p = part_at(plan, A, G, at, stop, blockIdx.x);
+        for (int at = begin; at < stop && ok;) {
+            const Part p = part_at(plan, A.T * G, G, at, stop, blockIdx.x);
             at = p.end;
+            // job j: tile j for warpgroup j & 1, or both warpgroups' halves of tile j / 2; scores run four jobs ahead
             const int nrt = p.rows > 128 ? 2 : 1, jobs = p.tiles * nrt;
             if (!(ok = wait_or_fail(&sy.qfull, qph, sy))) break;
             qph ^= 1;
-            tm_after();
-            for (int j = -2; j < jobs && ok; ++j) {
-                if (j >= 0) {  // the output's share of job j
-                    const int w = j & 1;
+#pragma unroll 1
+            for (int j = -4; j < jobs; ++j) {
+                if (j >= 0) {  // job j's share of the output
+                    const int w = j & 1, b = pcount[w] & 1;
                     if ((nrt == 1 || w == 0) && !(ok = wait_or_fail(&sy.vfull[vs], vph, sy))) break;
-                    if (!(ok = wait_or_fail(&sy.pready[w], pph[w], sy))) break;
-                    pph[w] ^= 1;
+                    if (!(ok = wait_or_fail(&sy.pready[w][b], (pcount[w] >> 1) & 1, sy))) break;
+                    ++pcount[w];
                     tm_after();
                     if (lane == 0) {
-                        const uint64_t b = desc_sw128(sv + vs * TILE, HALF);
+                        const uint64_t bv = v0 + (uint64_t)(vs * (TILE >> 4));
 #pragma unroll
                         for (int k = 0; k < KT / 16; ++k)
-                            mma_ts(tmem + 256 + w * 128, tmem + w * 128 + k * 8, b + k * (2048 >> 4), desc_o, j >= 2 || k > 0);
+                            mma_ts(tmem + 256 + w * 128, tmem + w * 128 + b * KT + k * 8, bv + k * (2048 >> 4), desc_o, j >= 2 || k > 0);
+                        mma_commit(smem_u32(&sy.pv[w][b]));
                         if (nrt == 1 || w == 1) mma_commit(smem_u32(&sy.vempty[vs]));
-                        if (j >= jobs - 2) mma_commit(smem_u32(&sy.odone[w]));
                     }
                     if (nrt == 1 || w == 1)
-                        if (++vs == X.vs) vs = 0, vph ^= 1;
+                        if (++vs == X.stages) vs = 0, vph ^= 1;
                 }
-                const int n = j + 2;
-                if (n < jobs) {  // the scores of job j + 2, over job j's
-                    const int w = n & 1;
+                const int n = j + 4;
+                if (n < jobs) {  // the scores of job j + 4, over the weights of the warpgroup's last but one
+                    const int w = n & 1, b = scount[w]++ & 1;
                     if ((nrt == 1 || w == 0) && !(ok = wait_or_fail(&sy.kfull[ks], kph, sy))) break;
                     tm_after();
                     if (lane == 0) {
-                        const uint64_t qa = desc_sw128(sq + (nrt == 2 ? w * TILE : 0), 0), kb = desc_sw128(sk + ks * TILE, 0);
+                        const uint64_t qa = q0 + (uint64_t)(nrt == 2 ? w * (QTILE >> 4) : 0), kb = k0 + (uint64_t)(ks * (TILE >> 4));
 #pragma unroll
-                        for (int k = 0; k < D / 16; ++k) {
-                            const uint64_t o = (uint64_t)(((k >> 2) * HALF + (k & 3) * 32) >> 4);
-                            mma_ss(tmem + w * 128, qa + o, kb + o, desc_s, k > 0);
-                        }
-                        mma_commit(smem_u32(&sy.sfull[w]));
+                        for (int k = 0; k < D / 16; ++k)
+                            mma_ss(tmem + w * 128 + b * KT, qa + (uint64_t)(((k >> 2) * QHALF + (k & 3) * 32) >> 4),
+                                   kb + (uint64_t)(((k >> 2) * HALF + (k & 3) * 32) >> 4), desc_s, k > 0);
+                        mma_commit(smem_u32(&sy.sfull[w][b]));
                         if (nrt == 1 || w == 1) mma_commit(smem_u32(&sy.kempty[ks]));
                     }
                     if (nrt == 1 || w == 1)
-                        if (++ks == X.ks) ks = 0, kph ^= 1;
+                        if (++ks == X.stages) ks = 0, kph ^= 1;
                 }
                 __syncwarp();
             }
@@ -754,25 +752,18 @@ struct States {
     long long p_row, u_row;
     int np, n, step, G;
     __device__ __forceinline__ States(const LongArgs& A, const Plan& P, int t, int g, int G_) : G(G_) {
-        const int lead = P.lead[t];
-        const long long all = (long long)P.tiles * A.Hk, tile = (long long)g * P.tiles + P.p_tile0[lead];
+        const int lead = P.lead[t], tile = g * P.tiles + P.p_tile0[lead];
+        const Cut cut(P.tiles * A.Hk, A.ctas);
         int c = 0;
         np = 0, step = A.T * G;
         if (P.p_tiles[lead] > 0) {
-            c = cta_of(A, all, tile);
-            np = cta_of(A, all, tile + P.p_tiles[lead] - 1) - c + 1;
+            c = cut.cta_of(tile);
+            np = cut.cta_of(tile + P.p_tiles[lead] - 1) - c + 1;
         }
         const int below = __popc(P.mask[lead] & ((1u << t) - 1u));  // the row's place among its prefix's
         p_row = (long long)c * step + (long long)g * P.rows + P.p_row0[lead] + below * G;
         u_row = A.unit_row + ((long long)g * P.units + P.unit0[t]) * G;
         n = np + (P.own_n[t] > 0 ? (P.own_n[t] + P.chunk - 1) / P.chunk : 0);
-    }
-    // the CTA whose stretch holds `tile`
-    static __device__ __forceinline__ int cta_of(const LongArgs& A, long long all, long long tile) {
-        int c = (int)(tile * min((long long)A.ctas, all) / all);
-        while (first_tile(all, c, A.ctas) > tile) --c;
-        while (first_tile(all, c + 1, A.ctas) <= tile) ++c;
-        return c;
     }
     __device__ __forceinline__ long long at(int k) const { return k < np ? p_row + (long long)k * step : u_row + (long long)(k - np) * G; }
 };
@@ -782,13 +773,15 @@ __device__ __forceinline__ void row_stats(const LongArgs& A, const States& S, in
     const int lane = threadIdx.x & 31;
     const float sink = A.sinks != nullptr ? __fmul_rn(A.sinks[head], LOG2E) : NEG_INF;
     M = sink;
-    for (int k = lane; k < S.n; k += 32) M = fmaxf(M, A.part_ml[S.at(k) + hh].x);
+    const float2 first = lane < S.n ? A.part_ml[S.at(lane) + hh] : make_float2(NEG_INF, 0.f);
+    M = fmaxf(M, first.x);
+    for (int k = lane + 32; k < S.n; k += 32) M = fmaxf(M, A.part_ml[S.at(k) + hh].x);
 #pragma unroll
     for (int k = 16; k > 0; k >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, k));
     const float sub = M == NEG_INF ? 0.f : M;
     L = 0.f;
     for (int k = lane; k < S.n; k += 32) {
-        const float2 ml = A.part_ml[S.at(k) + hh];
+        const float2 ml = k == lane ? first : A.part_ml[S.at(k) + hh];
         const float f = ml.x == NEG_INF ? 0.f : ex2(ml.x - sub);
         L += f * ml.y;
         if (fac != nullptr) fac[k] = f;
@@ -797,44 +790,38 @@ __device__ __forceinline__ void row_stats(const LongArgs& A, const States& S, in
     if (A.sinks != nullptr) L += ex2(sink - sub);
 }
 
-// The first T Hq blocks join one (row, query head) each: a warp every eighth state, a lane D / 32 dims, the warps' sums added
-// in order. The blocks after them, where a pass of few rows kept its scores, add up what it gives each cache row: a thread
-// a key, 2^(score - log2 of the row's denominator) over the kv head's queries in order - one sum in one order.
+// The first T Hk blocks join one (row, kv head) each: JW / G warps a query head, each every so many-th state, a lane D / 32
+// dims, their sums added in order. The blocks after them, where a pass of few rows kept its scores, add up what it gives each
+// cache row: a thread a key, 2^(score - log2 of the row's denominator) over the kv head's queries in order - one sum in one
+// order.
 template <int D, int G>
 __global__ void __launch_bounds__(JT) long_join(const LongArgs A, int weight_blocks) {
-    constexpr int E = D / 32;
+    constexpr int E = D / 32, WH = JW / G;  // warps a query head
     __shared__ Plan plan;
-    __shared__ float fac[STATES_MAX];
-    __shared__ float part[JW][D];
+    __shared__ float fac[JW][STATES_MAX];
+    __shared__ __align__(16) float part[JW][D];
     __shared__ float s_lse[KEEP_ROWS];
-    __shared__ float s_den;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     pdl_launch_dependents();
     if (warp == 0) make_plan(A, G, plan, false);
     __syncthreads();
-    if ((int)blockIdx.x < A.T * A.Hq) {
-        const int t = blockIdx.x / A.Hq, head = blockIdx.x - t * A.Hq, g = head / G, hh = head - g * G;
+    if ((int)blockIdx.x < A.T * A.Hk) {
+        const int t = blockIdx.x / A.Hk, g = blockIdx.x - t * A.Hk, hh = warp / WH, sub = warp - hh * WH, head = g * G + hh;
         if (plan.lead[t] < 0) {  // padding, or refused
             pdl_wait();
             return;
         }
         const States S(A, plan, t, g, G);
         pdl_wait();
-        if (warp == 0) {
-            float M, L;
-            row_stats(A, S, head, hh, M, L, fac);
-            if (lane == 0) {
-                s_den = L;
-                if (A.lse != nullptr) A.lse[(size_t)t * A.Hq + head] = M + log2f(L);
-            }
-        }
-        __syncthreads();
+        float M, L;
+        row_stats(A, S, head, hh, M, L, fac[warp]);
+        __syncwarp();
         float o[E];
 #pragma unroll
         for (int e = 0; e < E; ++e) o[e] = 0.f;
 #pragma unroll 4
-        for (int k = warp; k < S.n; k += JW) {
-            const float f = fac[k];
+        for (int k = sub; k < S.n; k += WH) {
+            const float f = fac[warp][k];
             const float* src = A.part_o + (size_t)(S.at(k) + hh) * D + lane * E;
             if (E == 4) {
                 const float4 v = *reinterpret_cast<const float4*>(src);
@@ -844,18 +831,27 @@ __global__ void __launch_bounds__(JT) long_join(const LongArgs A, int weight_blo
                 o[0] = fmaf(f, v.x, o[0]), o[E - 1] = fmaf(f, v.y, o[E - 1]);
             }
         }
+        if (WH > 1) {
 #pragma unroll
-        for (int e = 0; e < E; ++e) part[warp][lane * E + e] = o[e];
-        __syncthreads();
-        if (threadIdx.x < D) {
-            float a = 0.f;
-            for (int w = 0; w < min(JW, S.n); ++w) a += part[w][threadIdx.x];
-            A.out[(size_t)blockIdx.x * D + threadIdx.x] = f2bf(__fdiv_rn(a, s_den));
+            for (int e = 0; e < E; ++e) part[warp][lane * E + e] = o[e];
+            __syncthreads();
+            if (sub != 0) return;
+            for (int w = 1; w < min(WH, S.n); ++w)
+#pragma unroll
+                for (int e = 0; e < E; ++e) o[e] += part[warp + w][lane * E + e];
+        }
+        if (lane == 0 && A.lse != nullptr) A.lse[(size_t)t * A.Hq + head] = M + log2f(L);
+        bf16* out = A.out + ((size_t)t * A.Hq + head) * D + lane * E;
+#pragma unroll
+        for (int e = 0; e < E; e += 2) {
+            __nv_bfloat162 v;
+            v.x = f2bf(__fdiv_rn(o[e], L)), v.y = f2bf(__fdiv_rn(o[e + 1], L));
+            *reinterpret_cast<__nv_bfloat162*>(out + e) = v;
         }
         return;
     }
     // ---- the weights ------------------------------------------------------------------------------------------------------
-    const int b = blockIdx.x - A.T * A.Hq, g = b / weight_blocks, n = plan.n0 + (A.T == 1);  // keys whose scores were kept
+    const int b = blockIdx.x - A.T * A.Hk, g = b / weight_blocks, n = plan.n0 + (A.T == 1);  // keys whose scores were kept
     int j = (b - g * weight_blocks) * JT + threadIdx.x;
     pdl_wait();
     if (plan.lead[0] < 0 || (j - (int)threadIdx.x >= n && b != g * weight_blocks)) return;
@@ -994,9 +990,9 @@ int launch_tiles(const LongArgs& a, cudaStream_t s) {
     CUtensorMap tm[4];
     for (int k = 0; k < 4; ++k)
         if (const int rc = make_map(&tm[k], k < 2 ? a.K : a.V, rows, cols, a.rs, k & 1 ? 1 : KT)) return rc;
-    const int tile = KT * D * 2, nq = a.T * G > 128 ? 2 : 1, stages = (224 * 1024 - nq * tile) / tile;
-    x.vs = min(stages / 2, STAGES_MAX), x.ks = min(stages - x.vs, STAGES_MAX);
-    const size_t smem = (size_t)(nq + x.ks + x.vs) * tile;
+    const int tile = KT * D * 2, nq = a.T * G > 128 ? 2 : 1, queries = nq * 128 * D * 2;
+    x.stages = min((224 * 1024 - queries) / (2 * tile), STAGES_MAX);
+    const size_t smem = (size_t)queries + (size_t)2 * x.stages * tile;
     auto kern = long_tiles<D, G>;
     static bool allowed[64];
     if (const int rc = b2_allow_smem(reinterpret_cast<const void*>(kern), allowed)) return rc;
@@ -1007,7 +1003,7 @@ int launch_long(const LongArgs& a, cudaStream_t s) {
     if (const int rc = launch_tiles<D, G>(a, s)) return rc;
     // (blocks enough for a key a thread of the whole cache, or for the card)
     const int wb = a.scores != nullptr ? min((a.cap + JT - 1) / JT, max(1, 8 * a.ctas / a.Hk)) : 0;
-    if (const int rc = launch(long_join<D, G>, dim3(a.T * a.Hq + wb * a.Hk), dim3(JT), 0, s, a, wb)) return rc;
+    if (const int rc = launch(long_join<D, G>, dim3(a.T * a.Hk + wb * a.Hk), dim3(JT), 0, s, a, wb)) return rc;
     if (a.totals == nullptr || a.scores != nullptr) return B2_OK;
     auto kern = long_weights<D, G>;
     static bool allowed[64];
@@ -1036,6 +1032,7 @@ bool misaligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) !=
 int check_cache(const void* q, const void* K, const void* V, const void* out, int T, int Hq, int Hk, int D, long long hs,
                 long long rs, float scale, const void* workspace, int cap) {
     if (!shape_ok(T, Hq, Hk, D) || cap <= 0 || !(scale == scale) || hs < D || rs < D || (hs & 7) || (rs & 7)) return B2_ERR_DOMAIN;
+    if ((long long)cap * Hk > 0x7fffffffLL) return B2_ERR_DOMAIN;  // (tiles are counted in 32 bits)
     if (Hk > 1 && !((Hk - 1) * hs + D <= rs || (hs % rs == 0 && hs / rs >= cap))) return B2_ERR_DOMAIN;
     if (misaligned(q) || misaligned(K) || misaligned(V) || misaligned(out) || misaligned(workspace)) return B2_ERR_DOMAIN;
     return B2_OK;

@@ -116,6 +116,22 @@ def test_shared_rows_of_long_and_empty_prefixes(lens, live, step):
     assert capi.status() == 0
 
 
+@pytest.mark.parametrize("lens,live,Hq,Hk", [([30000], 32, 32, 4), ([20011, 9000], 31, 64, 8), ([40003], 3, 32, 8)])
+@pytest.mark.parametrize("D", [64, 128])
+def test_shared_rows_many_tiles_a_block(lens, live, Hq, Hk, D):
+    """long stretches of tiles a block, of 256 and of fewer query rows, several parts each; keys whose scores grow along the
+    cache, so that the running maximum moves often"""
+    g = gen(live + D)
+    T = E.pad_rows(live)
+    lay, cap = layout(live, T, lens, 40)
+    K, V, hs, rs = cache(g, cap, Hk, D)
+    K *= torch.linspace(0.2, 4, cap, device=DEV)[None, :, None].to(BF)
+    q = torch.randn(T, Hq, D, generator=g, device=DEV).to(BF)
+    got = shared(q, K, V, hs, rs, lay, cap)
+    check_shared(q, K, V, lay, got, live)
+    assert torch.equal(shared(q, K, V, hs, rs, lay, cap)[:live], got[:live]) and capi.status() == 0
+
+
 @pytest.mark.parametrize("win", [1, 7, 128, 500, 100000])
 @pytest.mark.parametrize("D", [64, 128])
 def test_shared_rows_windows_and_sinks(win, D):
