@@ -184,18 +184,44 @@ __device__ __forceinline__ uint64_t desc_sw128(uint32_t saddr, uint32_t lbo) {
     return (uint64_t)((saddr & 0x3FFFFu) >> 4) | ((uint64_t)(lbo >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) |
            ((uint64_t)2 << 61);
 }
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
-    asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d), "l"(a),
-                 "l"(b), "r"(idesc), "r"(acc)
+// The MMAs are issued by one elected lane (`lead` nonzero in it) of a warp whose lanes all walk the same code: the operands
+// then are warp-uniform values, which the instruction wants, and not one lane's.
+__device__ __forceinline__ uint32_t elect_lane() {
+    uint32_t on;
+    asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.u32 %0, 1, 0, p;\n}\n" : "=r"(on));
+    return on;
+}
+__device__ __forceinline__ void mma_ss(uint32_t lead, uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile("{\n.reg .pred p, q;\nsetp.ne.b32 p, %4, 0;\nsetp.ne.b32 q, %5, 0;\n"
+                 "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc), "r"(lead)
                  : "memory");
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
-    asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d), "r"(a),
-                 "l"(b), "r"(idesc), "r"(acc)
+__device__ __forceinline__ void mma_ts(uint32_t lead, uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile("{\n.reg .pred p, q;\nsetp.ne.b32 p, %4, 0;\nsetp.ne.b32 q, %5, 0;\n"
+                 "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(acc), "r"(lead)
                  : "memory");
 }
-__device__ __forceinline__ void mma_commit(uint32_t bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+__device__ __forceinline__ void mma_commit(uint32_t lead, uint32_t bar) {
+    asm volatile("{\n.reg .pred q;\nsetp.ne.b32 q, %1, 0;\n"
+                 "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}\n" ::"r"(bar), "r"(lead)
+                 : "memory");
+}
+// two f32 side by side: one instruction for both
+__device__ __forceinline__ uint64_t pair2(float x, float y) {
+    uint64_t v;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(x), "f"(y));
+    return v;
+}
+__device__ __forceinline__ void split2(uint64_t v, float& x, float& y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t v;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(v) : "l"(a), "l"(b), "l"(c));
+    return v;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t v;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b));
+    return v;
 }
 __device__ __forceinline__ void tm_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tm_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
@@ -279,16 +305,17 @@ struct TileArgs {
 };
 
 // a warp's bounded wait that also ends once any other role has given up; its lanes get one answer
+__device__ __noinline__ bool wait_long(uint32_t bar, uint32_t parity, TileSync& sy) {
+    for (uint32_t it = 0; it < B2_WAIT_LIMIT; ++it) {
+        if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+        if (__any_sync(0xffffffffu, *(volatile int*)&sy.fail)) return false;
+    }
+    *(volatile int*)&sy.fail = 1;
+    return false;
+}
 __device__ __forceinline__ bool wait_or_fail(uint64_t* bar, uint32_t parity, TileSync& sy) {
     const uint32_t b = smem_u32(bar);
-    bool ok = false;
-    uint32_t it = 0;
-    for (; it < B2_WAIT_LIMIT; ++it) {
-        if ((ok = mbar_try_wait(b, parity))) break;
-        if (*(volatile int*)&sy.fail) break;
-    }
-    if (it == B2_WAIT_LIMIT) *(volatile int*)&sy.fail = 1;
-    return __all_sync(0xffffffffu, ok);
+    return __all_sync(0xffffffffu, mbar_try_wait(b, parity)) || wait_long(b, parity, sy);
 }
 
 // a warp's units: every `stride`-th from `first` on. A lane a key for the scores and D / 32 dims for the output, a running
@@ -432,27 +459,19 @@ __global__ void __launch_bounds__(TW * 32, 1)
         sy.fail = 0;
         mbar_fence_init();
     }
+    if (warp == 9) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sy.tmem)), "r"(512u) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        tm_before();
+    }
     // the kernels before are through; only now may the joining kernel start, which reads what they left before it waits
     pdl_wait();
     pdl_launch_dependents();
     if (warp == 0) make_plan(A, G, plan, blockIdx.x == 0);
     __syncthreads();
     const Cut cut(plan.tiles * A.Hk, gridDim.x);
-    const int begin = cut.first(blockIdx.x), stop = cut.first(blockIdx.x + 1);
-    if (begin >= stop) {  // no tiles for this CTA: nothing allocated yet
-        if (warp >= 10) own_units<D, G>(A, plan, (warp - 10) * gridDim.x + blockIdx.x, OWN_WARPS * gridDim.x);
-        return;
-    }
-    if (sq & 1023) {  // (the tiles take all but 3 KB of what a block may have: there is no room to align them here)
-        if (threadIdx.x == 0) b2_fail(B2_ERR_CUDA);
-        return;
-    }
-    if (warp == 9) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sy.tmem)), "r"(512u) : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-    }
-    tm_before();
-    __syncthreads();
+    const int begin = cut.first(blockIdx.x);
+    const int stop = sq & 1023 ? begin : cut.first(blockIdx.x + 1);  // (the tiles leave no room to align them here)
     tm_after();
     const uint32_t tmem = sy.tmem;
 
@@ -546,20 +565,24 @@ __global__ void __launch_bounds__(TW * 32, 1)
                                 make_float4(__uint_as_float(s[c >> 5][c & 31]) * scale2, __uint_as_float(s[c >> 5][(c & 31) + 1]) * scale2,
                                             __uint_as_float(s[c >> 5][(c & 31) + 2]) * scale2, __uint_as_float(s[c >> 5][(c & 31) + 3]) * scale2);
                     }
-                    float sum[4] = {0.f, 0.f, 0.f, 0.f};
+                    const uint64_t mul = pair2(scale2, scale2), add = pair2(-sub, -sub);
+                    uint64_t sum[2] = {0ull, 0ull};  // (two sums each)
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
                         uint32_t w[16];
 #pragma unroll
                         for (int c = 0; c < 16; ++c) {
-                            const float x = ex2(fmaf(__uint_as_float(s[h][2 * c]), scale2, -sub));
-                            const float y = ex2(fmaf(__uint_as_float(s[h][2 * c + 1]), scale2, -sub));
-                            sum[(2 * c) & 3] += x, sum[(2 * c + 1) & 3] += y;
+                            float x, y;
+                            split2(fma2(pair2(__uint_as_float(s[h][2 * c]), __uint_as_float(s[h][2 * c + 1])), mul, add), x, y);
+                            x = ex2(x), y = ex2(y);
+                            sum[c & 1] = add2(sum[c & 1], pair2(x, y));
                             asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w[c]) : "f"(y), "f"(x));
                         }
                         tm_st16(ts + b * KT + h * 16, w);
                     }
-                    l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                    float x, y;
+                    split2(add2(sum[0], sum[1]), x, y);
+                    l += x + y;
                     tm_wait_st();
                 }
                 tm_before();
@@ -681,64 +704,60 @@ __global__ void __launch_bounds__(TW * 32, 1)
         constexpr uint32_t base_desc = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(128 >> 4) << 24);
         constexpr uint32_t desc_s = base_desc | ((uint32_t)(KT >> 3) << 17), desc_o = base_desc | (1u << 16) | ((uint32_t)(D >> 3) << 17);
         const uint64_t q0 = desc_sw128(sq, 0), k0 = desc_sw128(sk, 0), v0 = desc_sw128(sv, HALF);
+        const uint32_t lead = elect_lane();
         int ks = 0, vs = 0;
-        uint32_t kph = 0, vph = 0, qph = 0, scount[2] = {0, 0}, pcount[2] = {0, 0};
+        uint32_t kph = 0, vph = 0, qph = 0, scount0 = 0, scount1 = 0, pcount0 = 0, pcount1 = 0;
         bool ok = true;
         for (int at = begin; at < stop && ok;) {
             const Part p = part_at(plan, A.T * G, G, at, stop, blockIdx.x);
-            at = p.end;
+            at = __shfl_sync(0xffffffffu, p.end, 0);
             // job j: tile j for warpgroup j & 1, or both warpgroups' halves of tile j / 2; scores run four jobs ahead
-            const int nrt = p.rows > 128 ? 2 : 1, jobs = p.tiles * nrt;
+            const int nrt = __shfl_sync(0xffffffffu, p.rows, 0) > 128 ? 2 : 1, jobs = __shfl_sync(0xffffffffu, p.tiles, 0) * nrt;
             if (!(ok = wait_or_fail(&sy.qfull, qph, sy))) break;
             qph ^= 1;
 #pragma unroll 1
             for (int j = -4; j < jobs; ++j) {
+                const int w = j & 1;  // (job j + 4's warpgroup too)
+                const bool begins = nrt == 1 || w == 0, ends = nrt == 1 || w == 1;  // its tile's first, last job
                 if (j >= 0) {  // job j's share of the output
-                    const int w = j & 1, b = pcount[w] & 1;
-                    if ((nrt == 1 || w == 0) && !(ok = wait_or_fail(&sy.vfull[vs], vph, sy))) break;
-                    if (!(ok = wait_or_fail(&sy.pready[w][b], (pcount[w] >> 1) & 1, sy))) break;
-                    ++pcount[w];
+                    const uint32_t c = w ? pcount1++ : pcount0++, b = c & 1;
+                    if (begins && !(ok = wait_or_fail(&sy.vfull[vs], vph, sy))) break;
+                    if (!(ok = wait_or_fail(&sy.pready[w][b], (c >> 1) & 1, sy))) break;
                     tm_after();
-                    if (lane == 0) {
-                        const uint64_t bv = v0 + (uint64_t)(vs * (TILE >> 4));
+                    const uint64_t bv = v0 + (uint64_t)(vs * (TILE >> 4));
 #pragma unroll
-                        for (int k = 0; k < KT / 16; ++k)
-                            mma_ts(tmem + 256 + w * 128, tmem + w * 128 + b * KT + k * 8, bv + k * (2048 >> 4), desc_o, j >= 2 || k > 0);
-                        mma_commit(smem_u32(&sy.pv[w][b]));
-                        if (nrt == 1 || w == 1) mma_commit(smem_u32(&sy.vempty[vs]));
-                    }
-                    if (nrt == 1 || w == 1)
+                    for (int k = 0; k < KT / 16; ++k)
+                        mma_ts(lead, tmem + 256 + w * 128, tmem + w * 128 + b * KT + k * 8, bv + k * (2048 >> 4), desc_o, j >= 2 || k > 0);
+                    mma_commit(lead, smem_u32(&sy.pv[w][b]));
+                    if (ends) {
+                        mma_commit(lead, smem_u32(&sy.vempty[vs]));
                         if (++vs == X.stages) vs = 0, vph ^= 1;
-                }
-                const int n = j + 4;
-                if (n < jobs) {  // the scores of job j + 4, over the weights of the warpgroup's last but one
-                    const int w = n & 1, b = scount[w]++ & 1;
-                    if ((nrt == 1 || w == 0) && !(ok = wait_or_fail(&sy.kfull[ks], kph, sy))) break;
-                    tm_after();
-                    if (lane == 0) {
-                        const uint64_t qa = q0 + (uint64_t)(nrt == 2 ? w * (QTILE >> 4) : 0), kb = k0 + (uint64_t)(ks * (TILE >> 4));
-#pragma unroll
-                        for (int k = 0; k < D / 16; ++k)
-                            mma_ss(tmem + w * 128 + b * KT, qa + (uint64_t)(((k >> 2) * QHALF + (k & 3) * 32) >> 4),
-                                   kb + (uint64_t)(((k >> 2) * HALF + (k & 3) * 32) >> 4), desc_s, k > 0);
-                        mma_commit(smem_u32(&sy.sfull[w][b]));
-                        if (nrt == 1 || w == 1) mma_commit(smem_u32(&sy.kempty[ks]));
                     }
-                    if (nrt == 1 || w == 1)
-                        if (++ks == X.stages) ks = 0, kph ^= 1;
                 }
-                __syncwarp();
+                if (j + 4 < jobs) {  // the scores of job j + 4, over the weights of the warpgroup's last but one
+                    const uint32_t b = (w ? scount1++ : scount0++) & 1;
+                    if (begins && !(ok = wait_or_fail(&sy.kfull[ks], kph, sy))) break;
+                    tm_after();
+                    const uint64_t qa = q0 + (uint64_t)(nrt == 2 ? w * (QTILE >> 4) : 0), kb = k0 + (uint64_t)(ks * (TILE >> 4));
+#pragma unroll
+                    for (int k = 0; k < D / 16; ++k)
+                        mma_ss(lead, tmem + w * 128 + b * KT, qa + (uint64_t)(((k >> 2) * QHALF + (k & 3) * 32) >> 4),
+                               kb + (uint64_t)(((k >> 2) * HALF + (k & 3) * 32) >> 4), desc_s, k > 0);
+                    mma_commit(lead, smem_u32(&sy.sfull[w][b]));
+                    if (ends) {
+                        mma_commit(lead, smem_u32(&sy.kempty[ks]));
+                        if (++ks == X.stages) ks = 0, kph ^= 1;
+                    }
+                }
             }
         }
-        if (lane == 0) {
-            mma_commit(smem_u32(&sy.drain));
-            (void)mbar_wait_bounded(smem_u32(&sy.drain), 0);
-        }
+        mma_commit(lead, smem_u32(&sy.drain));
+        (void)mbar_wait_bounded(smem_u32(&sy.drain), 0);
         __syncwarp();
     }
     tm_before();
     __syncthreads();
-    if (threadIdx.x == 0 && sy.fail) b2_fail(B2_ERR_TIMEOUT);
+    if (threadIdx.x == 0 && (sy.fail || (sq & 1023))) b2_fail(sy.fail ? B2_ERR_TIMEOUT : B2_ERR_CUDA);
     if (warp == 9) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
 }
 
