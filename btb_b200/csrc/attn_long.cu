@@ -897,53 +897,140 @@ __global__ void __launch_bounds__(JT) long_join(const LongArgs A, int weight_blo
     }
 }
 
-constexpr int WK = 128;  // keys of a weights block
-
-// What the pass gives each cache row: a thread a key, its score against every row's query again and the weights
-// 2^(score - lse) added in row order, so that a total is one sum in one order. The pass's own rows are set, not added to.
-template <int D, int G>
-__global__ void __launch_bounds__(WK) long_weights(const LongArgs A) {
-    extern __shared__ __align__(16) uint32_t dyn[];  // the kv head's queries, [T * G][D / 2]
-    pdl_launch_dependents();
-    pdl_wait();
-    const int g = blockIdx.y, n0 = *A.n0p, j = blockIdx.x * WK + threadIdx.x;
-    if (n0 < 0 || n0 > A.cap - A.T) return;
-    float* tot = A.totals + (size_t)g * A.ts;
-    if (blockIdx.x == 0 && threadIdx.x < A.T) {
-        float a = 0.f;
-        for (int t = 0; t < A.T; ++t)
-            for (int hh = 0; hh < G; ++hh) {
-                const size_t r = (size_t)t * A.Hq + g * G + hh;
-                a += ex2(A.own[r * 32 + threadIdx.x] - A.lse[r]);
-            }
-        tot[n0 + threadIdx.x] = a;
+// ---- what a pass of many rows gives each cache row -------------------------------------------------------------------------
+// The scores once more, turned round: S^T = K Q^T with 128 keys as the MMA's M and the kv head's T G queries as its N, so that
+// a thread has a key and adds the weights 2^(score - log2 of the row's denominator) of its row of tensor memory one after the
+// other - one sum in one order, no exchange. Bound by the powers (a tile of 128 keys and 256 queries: 32768, 16 a clock) once
+// there are tiles for every SM; the queries, the first tile and its product are ready before the joining kernel is waited for.
+constexpr int WT = 128;  // keys of a tile, threads of a block
+template <int D>
+__global__ void __launch_bounds__(WT) long_weights(const __grid_constant__ CUtensorMap kbox, const __grid_constant__ CUtensorMap krows,
+                                                   const TileArgs X) {
+    constexpr int TILE = WT * D * 2, HALF = WT * 128;
+    const LongArgs& A = X.a;
+    extern __shared__ __align__(1024) uint8_t smem[];
+    __shared__ __align__(8) uint64_t full, done;
+    __shared__ uint32_t tmem_slot;
+    __shared__ float s_lse[256];
+    const int G = A.Hq / A.Hk, rows = A.T * G, N = (rows + 31) & ~31, g = blockIdx.y;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t sk = smem_u32(smem), sq = sk + TILE, cols = N > 128 ? 256u : N > 64 ? 128u : N > 32 ? 64u : 32u;
+    const int n0 = *A.n0p;
+    const bool fits = n0 >= 0 && n0 <= A.cap - A.T && !(sk & 1023);
+    const int tiles = fits ? (n0 + WT - 1) / WT : 0;
+    if ((sk & 1023) && threadIdx.x == 0) b2_fail(B2_ERR_CUDA);
+    if (!fits || ((int)blockIdx.x >= tiles && blockIdx.x > 0)) {
+        pdl_launch_dependents();
+        pdl_wait();
+        return;
     }
-    if ((int)blockIdx.x * WK >= n0) return;
-    for (int i = threadIdx.x; i < A.T * G * (D / 2); i += WK) {
-        const int r = i / (D / 2), d = i - r * (D / 2);
-        dyn[i] = reinterpret_cast<const uint32_t*>(A.q + ((size_t)(r / G) * A.Hq + g * G + r % G) * D)[d];
+    if (threadIdx.x == 0) {
+        mbar_init(smem_u32(&full), 1), mbar_init(smem_u32(&done), 1);
+        mbar_fence_init();
     }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(cols) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tm_before();
     __syncthreads();
-    if (j >= n0) return;
-    const int row = A.tbl != nullptr ? A.tbl[j] : j;
-    if (row < 0 || row >= A.cap) return;  // refused by the pass over the rows
-    uint4 kv[D / 8];
-    const uint4* kr = reinterpret_cast<const uint4*>(A.K + (size_t)g * A.hs + (size_t)row * A.rs);
-#pragma unroll
-    for (int c = 0; c < D / 8; ++c) kv[c] = __ldg(kr + c);
-    const float scale2 = __fmul_rn(A.scale, LOG2E);
-    float a = 0.f;
-    for (int r = 0; r < A.T * G; ++r) {
-        const uint4* q4 = reinterpret_cast<const uint4*>(dyn + r * (D / 2));
-        float s = 0.f;
-#pragma unroll
-        for (int c = 0; c < D / 8; ++c) {
-            const uint4 w = q4[c];
-            s = fma2_bf16(kv[c].w, w.w, fma2_bf16(kv[c].z, w.z, fma2_bf16(kv[c].y, w.y, fma2_bf16(kv[c].x, w.x, s))));
+    tm_after();
+    pdl_launch_dependents();
+    const uint32_t tmem = tmem_slot;
+    const int x = g * X.col_mul, y0 = g * X.row_mul;
+    auto load = [&](int tile) {  // (warp 0)
+        const int keys = min(WT, n0 - tile * WT);
+        const uint32_t bar = smem_u32(&full);
+        if (lane == 0) mbar_expect_tx(bar, TILE);
+        __syncwarp();
+        if (keys == WT && A.tbl == nullptr) {
+            if (lane < D / 32) tma_box(sk + lane * (KT * 128), &kbox, x + (lane >> 1) * 64, y0 + tile * WT + (lane & 1) * KT, bar);
+            return;
         }
-        a += ex2(__fmul_rn(s, scale2) - A.lse[(size_t)(r / G) * A.Hq + g * G + r % G]);
+        int y[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int j = tile * WT + min(lane * 4 + k, keys - 1);
+            const int r = A.tbl != nullptr ? A.tbl[j] : j;
+            y[k] = y0 + (r < 0 || r >= A.cap ? 0 : r);  // (refused by the tiles' kernel)
+        }
+        for (int c = 0; c < D / 64; ++c) tma_rows4(sk + c * HALF + lane * 512, &krows, x + c * 64, y, bar);
+    };
+    if (warp == 0 && tiles > 0) load(blockIdx.x);
+    for (int i = threadIdx.x; i < rows * (D / 8); i += WT) {
+        const int r = i / (D / 8), piece = i - r * (D / 8), t = r / G;
+        const uint4 v = reinterpret_cast<const uint4*>(A.q + ((size_t)t * A.Hq + g * G + r - t * G) * D)[piece];
+        *reinterpret_cast<uint4*>(smem + TILE + (piece >> 3) * (N * 128) + r * 128 + (((piece & 7) ^ (r & 7)) << 4)) = v;
     }
-    tot[j] += a;
+    fence_proxy_async();
+    __syncthreads();
+    const float scale2 = __fmul_rn(A.scale, LOG2E);
+    float* tot = A.totals + (size_t)g * A.ts;
+    bool ok = true, first = true;
+    uint32_t ph = 0;
+    for (int tile = blockIdx.x; first || tile < tiles; tile += gridDim.x, ph ^= 1) {
+        if (warp == 0 && tile < tiles) {
+            ok = mbar_wait_bounded(smem_u32(&full), ph);
+            ok = __all_sync(0xffffffffu, ok);
+            if (ok) {
+                const uint32_t lead = elect_lane();
+                const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(WT >> 4) << 24);
+                const uint64_t ka = desc_sw128(sk, 0), qb = desc_sw128(sq, 0);
+                tm_after();
+#pragma unroll
+                for (int k = 0; k < D / 16; ++k)
+                    mma_ss(lead, tmem, ka + (uint64_t)(((k >> 2) * HALF + (k & 3) * 32) >> 4),
+                           qb + (uint64_t)(((k >> 2) * (N * 128) + (k & 3) * 32) >> 4), idesc, k > 0);
+                mma_commit(lead, smem_u32(&done));
+            }
+        }
+        if (first) {  // everything so far was there before the tiles; the denominators are the joining kernel's
+            pdl_wait();
+            for (int r = threadIdx.x; r < rows; r += WT) s_lse[r] = A.lse[(size_t)(r / G) * A.Hq + g * G + r % G];
+            __syncthreads();
+            if (blockIdx.x == 0 && (int)threadIdx.x < A.T) {  // the pass's own rows: set
+                float a = 0.f;
+#pragma unroll 8
+                for (int r = 0; r < rows; ++r) a += ex2(A.own[((size_t)(r / G) * A.Hq + g * G + r % G) * 32 + threadIdx.x] - s_lse[r]);
+                tot[n0 + threadIdx.x] = a;
+            }
+            first = false;
+        }
+        if (tile >= tiles) break;
+        if (ok) ok = mbar_wait_bounded(smem_u32(&done), ph);
+        if (!__syncthreads_and(ok)) break;
+        tm_after();
+        if (warp == 0 && tile + (int)gridDim.x < tiles) load(tile + gridDim.x);  // (the product has read this one)
+        float a = 0.f;
+        const uint32_t at = tmem + ((uint32_t)(warp * 32) << 16);
+#pragma unroll 1
+        for (int c0 = 0; c0 < N; c0 += 32) {
+            uint32_t s[32];
+            tm_ld32(at + c0, s);
+            tm_wait_ld(s);
+            const int n = min(32, rows - c0);
+            if (n == 32) {
+                float e[32];
+#pragma unroll
+                for (int c = 0; c < 32; ++c) e[c] = ex2(fmaf(__uint_as_float(s[c]), scale2, -s_lse[c0 + c]));
+#pragma unroll
+                for (int c = 0; c < 32; ++c) a += e[c];
+            } else {
+#pragma unroll
+                for (int c = 0; c < 32; ++c)
+                    if (c < n) a += ex2(fmaf(__uint_as_float(s[c]), scale2, -s_lse[c0 + c]));
+            }
+        }
+        const int j = tile * WT + threadIdx.x;
+        if (j < n0) tot[j] += a;
+        tm_before();
+        __syncthreads();
+        tm_after();
+    }
+    if (!ok) b2_fail(B2_ERR_TIMEOUT);
+    tm_before();
+    __syncthreads();
+    if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(cols) : "memory");
 }
 
 typedef CUresult (*EncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
@@ -999,7 +1086,7 @@ long long score_stride(int cap) { return ((long long)cap + KT - 1) / KT * KT; }
 bool keeps_scores(int T, int Hq, int Hk) { return T * (Hq / Hk) <= KEEP_ROWS; }
 
 template <int D, int G>
-int launch_tiles(const LongArgs& a, cudaStream_t s) {
+int launch_long(const LongArgs& a, cudaStream_t s) {
     TileArgs x{};
     x.a = a;
     const bool by_row = a.Hk == 1 || (a.Hk - 1) * a.hs + D <= a.rs;  // kv heads inside a cache row
@@ -1009,25 +1096,21 @@ int launch_tiles(const LongArgs& a, cudaStream_t s) {
     CUtensorMap tm[4];
     for (int k = 0; k < 4; ++k)
         if (const int rc = make_map(&tm[k], k < 2 ? a.K : a.V, rows, cols, a.rs, k & 1 ? 1 : KT)) return rc;
-    const int tile = KT * D * 2, nq = a.T * G > 128 ? 2 : 1, queries = nq * 128 * D * 2;
+    const int tile = KT * D * 2, queries = (a.T * G > 128 ? 2 : 1) * 128 * D * 2;
     x.stages = min((224 * 1024 - queries) / (2 * tile), STAGES_MAX);
-    const size_t smem = (size_t)queries + (size_t)2 * x.stages * tile;
-    auto kern = long_tiles<D, G>;
-    static bool allowed[64];
-    if (const int rc = b2_allow_smem(reinterpret_cast<const void*>(kern), allowed)) return rc;
-    return launch(kern, dim3(a.ctas), dim3(TW * 32), smem, s, tm[0], tm[1], tm[2], tm[3], x);
-}
-template <int D, int G>
-int launch_long(const LongArgs& a, cudaStream_t s) {
-    if (const int rc = launch_tiles<D, G>(a, s)) return rc;
+    auto tiles = long_tiles<D, G>;
+    static bool tiles_allowed[64], weights_allowed[64];
+    if (const int rc = b2_allow_smem(reinterpret_cast<const void*>(tiles), tiles_allowed)) return rc;
+    if (const int rc = launch(tiles, dim3(a.ctas), dim3(TW * 32), (size_t)queries + (size_t)2 * x.stages * tile, s, tm[0], tm[1], tm[2], tm[3], x))
+        return rc;
     // (blocks enough for a key a thread of the whole cache, or for the card)
     const int wb = a.scores != nullptr ? min((a.cap + JT - 1) / JT, max(1, 8 * a.ctas / a.Hk)) : 0;
     if (const int rc = launch(long_join<D, G>, dim3(a.T * a.Hk + wb * a.Hk), dim3(JT), 0, s, a, wb)) return rc;
     if (a.totals == nullptr || a.scores != nullptr) return B2_OK;
-    auto kern = long_weights<D, G>;
-    static bool allowed[64];
-    if (const int rc = b2_allow_smem(reinterpret_cast<const void*>(kern), allowed)) return rc;
-    return launch(kern, dim3((a.cap + WK - 1) / WK, a.Hk), dim3(WK), (size_t)a.T * G * D * 2, s, a);
+    auto weights = long_weights<D>;
+    if (const int rc = b2_allow_smem(reinterpret_cast<const void*>(weights), weights_allowed)) return rc;
+    const int N = (a.T * G + 31) & ~31;  // two blocks an SM
+    return launch(weights, dim3(min((a.cap + WT - 1) / WT, max(1, 2 * a.ctas / a.Hk)), a.Hk), dim3(WT), (size_t)(WT + N) * D * 2, s, tm[0], tm[1], x);
 }
 template <int D>
 int launch_long_g(const LongArgs& a, cudaStream_t s) {

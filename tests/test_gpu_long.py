@@ -276,7 +276,7 @@ def test_scored_equals_the_definition(D, Hq, Hk, T, n0, par):
 
 
 @pytest.mark.parametrize("kind", ["rows", "wide", "heads"])
-@pytest.mark.parametrize("T,n0", [(1, 20000), (5, 4097)])
+@pytest.mark.parametrize("T,n0", [(1, 20000), (5, 4097), (2, 9000), (32, 30011)])
 def test_scored_long_paged_sinks_and_layouts(kind, T, n0):
     g = gen(n0 + T)
     Hq, Hk, D, cap = 16, 2, 128, (n0 + T + 70) // 64 * 64
