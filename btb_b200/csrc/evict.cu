@@ -1,6 +1,9 @@
 // Eviction from a cache by accumulated attention weight, for sm_100a: per (layer, kv head) the `recent` last rows stay,
 // and of the others the keep - recent with the largest totals, the lower row first among equals. The kept rows move
 // down in order, their keys, values and totals with them, in place or into another cache.
+//
+// Two launches. evict_pick: a block a (layer, kv head) finds the rows from its totals and moves those. evict_move: the keys
+// and values, bound by memory - every kept row read and written once.
 #include "common.cuh"
 #include "btb_b200_internal.h"
 
@@ -25,157 +28,200 @@ struct EvictArgs {
     int* n_seen;          // n0 as the selection read it (n_out may be n0p's word)
     long long ls, ld, hs, rs;
     int layers, Hk, D, cap, cap_d, keep, recent;
+    int held;             // the totals of a head fit a block's shared memory
+    int parts;            // evict_move: blocks that share a (layer, kv head, K or V): pieces of a row in place, else ranges of rows
+    int in_place;
 };
 
 // a total's rank as an unsigned word: larger totals rank higher, -0 as 0, every NaN above all else
-__device__ __forceinline__ uint32_t rank_of(float v) {
+__device__ __forceinline__ uint32_t rank_of(uint32_t bits) {
+    const float v = __uint_as_float(bits);
     if (v != v) return 0xffffffffu;
     const uint32_t b = __float_as_uint(v + 0.f);
     return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
 }
 
-constexpr int ST = 1024;  // threads of a selection block
+constexpr int ST = 1024, SW = ST / 32;  // threads and warps of a selection block
+constexpr int BINS = 2048;              // eleven bits of the rank at a time: 11, 11, 10
 
-// inclusive sums over a block's threads; every thread gets its own and the block's
-__device__ __forceinline__ int block_scan(int v, int* warp_sums, int& total) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const int u = __shfl_up_sync(0xffffffffu, v, o);
-        if (lane >= o) v += u;
-    }
-    if (lane == 31) warp_sums[warp] = v;
-    __syncthreads();
-    if (warp == 0) {
-        int w = warp_sums[lane];
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int u = __shfl_up_sync(0xffffffffu, w, o);
-            if (lane >= o) w += u;
-        }
-        warp_sums[lane] = w;
-    }
-    __syncthreads();
-    total = warp_sums[31];
-    const int before = warp > 0 ? warp_sums[warp - 1] : 0;
-    __syncthreads();
-    return v + before;
-}
-
-// the kept rows of one (layer, kv head): the rank of the last kept total found a byte at a time from histograms, then one
-// ordered pass that writes the rows above it and as many equal to it, from the lowest on, as there is room for
+// The rank of the last kept total, eleven bits at a time from histograms of the totals that share the bits above (a warp
+// adds the lanes of a bin at once: many rows have equal totals); then the rows above it and, from the lowest on, as many
+// equal to it as there is room for - each warp counts a stretch of rows, and writes it behind the stretches before it.
+// The totals are read once into shared memory where they fit (48 K rows), else again in each of the five passes.
 __global__ void __launch_bounds__(ST) evict_pick(const EvictArgs A) {
-    __shared__ unsigned hist[256];
-    __shared__ int warp_sums[32];
-    __shared__ unsigned s_digit;
-    __shared__ int s_left;
-    pdl_launch_dependents();
+    extern __shared__ uint32_t held[];
+    __shared__ int hist[BINS];
+    __shared__ int sums[2][SW];
+    __shared__ int s_bin, s_left;
     pdl_wait();
+    pdl_launch_dependents();
     const int g = blockIdx.x, a = blockIdx.y, n = *A.n0p;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const bool bad = n < 0 || n > A.cap;
     if (threadIdx.x == 0 && g == 0 && a == 0) {
-        *A.n_seen = bad ? 0 : n;
+        *A.n_seen = bad ? -1 : n;
         if (bad) b2_fail(B2_ERR_DOMAIN);
     }
     if (bad) return;
-    const float* tot = A.totals + ((size_t)a * A.Hk + g) * A.cap;
-    int* idx = A.idx + ((size_t)a * A.Hk + g) * A.keep;
-    for (int i = threadIdx.x; i < A.keep; i += ST) {
-        if (n <= A.keep) idx[i] = i < n ? i : -1;
-        else if (i >= A.keep - A.recent) idx[i] = n - A.keep + i;
+    const size_t head = (size_t)a * A.Hk + g;
+    const uint32_t* tot = reinterpret_cast<const uint32_t*>(A.totals) + head * A.cap;
+    uint32_t* tot_d = reinterpret_cast<uint32_t*>(A.totals_d) + head * A.cap_d;
+    int* idx = A.idx + head * A.keep;
+    const int want = A.keep - A.recent, from = n - A.recent;  // rows to be found, among rows 0 .. from - 1
+    if (n <= A.keep) {
+        for (int i = threadIdx.x; i < A.keep; i += ST) {
+            idx[i] = i < n ? i : -1;
+            if (i < n && !A.in_place) tot_d[i] = tot[i];
+        }
+        return;
     }
-    const int want = A.keep - A.recent, from = n - A.recent;
-    if (n <= A.keep || want == 0) return;
-    unsigned prefix = 0, mask = 0;
-    int left = want;  // rows still to be found among those that share `prefix`
-    for (int shift = 24; shift >= 0; shift -= 8) {
-        for (int i = threadIdx.x; i < 256; i += ST) hist[i] = 0;
-        __syncthreads();
-        for (int j = threadIdx.x; j < from; j += ST) {
-            const uint32_t k = rank_of(tot[j]);
-            if ((k & mask) == prefix) atomicAdd(&hist[(k >> shift) & 255], 1u);
-        }
-        __syncthreads();
-        if (threadIdx.x == 0) {
-            int d = 255, l = left;
-            while (d > 0 && (int)hist[d] < l) l -= hist[d--];
-            s_digit = d, s_left = l;
-        }
-        __syncthreads();
-        prefix |= s_digit << shift, mask |= 255u << shift;
-        left = s_left;
+    if (A.held) {
+#pragma unroll 8
+        for (int j = threadIdx.x; j < n; j += ST) held[j] = tot[j];
         __syncthreads();
     }
-    int done = 0, ties = 0;  // rows written, rows equal to the last kept total seen
-    for (int j0 = 0; j0 < from; j0 += ST) {
-        const int j = j0 + threadIdx.x;
-        const uint32_t k = j < from ? rank_of(tot[j]) : 0u;
-        const bool tie = j < from && k == prefix;
-        int n_tie, n_kept;
-        const int tie_at = block_scan(tie, warp_sums, n_tie);
-        const bool in = j < from && (k > prefix || (tie && ties + tie_at <= left));
-        const int at = block_scan(in, warp_sums, n_kept);
-        if (in) idx[done + at - 1] = j;
-        done += n_kept, ties += n_tie;
+    auto bits = [&](int j) { return A.held ? held[j] : __ldcg(tot + j); };
+    if (want > 0) {
+        uint32_t prefix = 0, mask = 0;
+        int left = want;  // rows still to be found among those that share `prefix`
+#pragma unroll 1
+        for (int step = 0; step < 3; ++step) {
+            const int shift = step == 0 ? 21 : step == 1 ? 10 : 0;
+            const uint32_t field = step == 2 ? 1023u : 2047u;
+            for (int i = threadIdx.x; i < BINS; i += ST) hist[i] = 0;
+            __syncthreads();
+            for (int j0 = warp * 32; j0 < from; j0 += ST) {
+                const int j = j0 + lane;
+                const uint32_t k = j < from ? rank_of(bits(j)) : 0u;
+                const bool on = j < from && (k & mask) == prefix;
+                const unsigned active = __ballot_sync(0xffffffffu, on);
+                if (on) {
+                    const uint32_t bin = (k >> shift) & field;
+                    const unsigned same = __match_any_sync(active, bin);
+                    if (lane == __ffs(same) - 1) atomicAdd(&hist[bin], __popc(same));
+                }
+            }
+            __syncthreads();
+            // thread i: bins 2047 - 2 i and the one below; how many rows lie in them and above
+            const int hi = hist[BINS - 1 - 2 * threadIdx.x], lo = hist[BINS - 2 - 2 * threadIdx.x];
+            int v = hi + lo;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int u = __shfl_up_sync(0xffffffffu, v, o);
+                if (lane >= o) v += u;
+            }
+            if (lane == 31) sums[0][warp] = v;
+            __syncthreads();
+            int before = warp > 0 && lane < warp ? sums[0][lane] : 0;
+            before = __reduce_add_sync(0xffffffffu, before) + v - hi - lo;
+            if (before < left && left <= before + hi) s_bin = BINS - 1 - 2 * threadIdx.x, s_left = left - before;
+            else if (before + hi < left && left <= before + hi + lo) s_bin = BINS - 2 - 2 * threadIdx.x, s_left = left - before - hi;
+            __syncthreads();
+            prefix |= (uint32_t)s_bin << shift, mask |= field << shift;
+            left = s_left;
+        }
+        // each warp's stretch: rows above the last kept rank, rows equal to it
+        const int per = ((from + SW - 1) / SW + 31) & ~31, j_lo = min(warp * per, from), j_hi = min(j_lo + per, from);
+        int above = 0, equal = 0;
+        for (int j0 = j_lo; j0 < j_hi; j0 += 32) {
+            const uint32_t k = j0 + lane < j_hi ? rank_of(bits(j0 + lane)) : 0u;
+            above += __popc(__ballot_sync(0xffffffffu, j0 + lane < j_hi && k > prefix));
+            equal += __popc(__ballot_sync(0xffffffffu, j0 + lane < j_hi && k == prefix));
+        }
+        __syncthreads();
+        if (lane == 0) sums[0][warp] = above, sums[1][warp] = equal;
+        __syncthreads();
+        int ties = __reduce_add_sync(0xffffffffu, lane < warp ? sums[1][lane] : 0);  // equal rows before the stretch
+        int at = __reduce_add_sync(0xffffffffu, lane < warp ? sums[0][lane] : 0) + min(ties, left);
+        for (int j0 = j_lo; j0 < j_hi; j0 += 32) {
+            const int j = j0 + lane;
+            const uint32_t k = j < j_hi ? rank_of(bits(j)) : 0u;
+            const unsigned eq = __ballot_sync(0xffffffffu, j < j_hi && k == prefix), below = (1u << lane) - 1u;
+            const bool in = j < j_hi && (k > prefix || (k == prefix && ties + __popc(eq & below) < left));
+            const unsigned kept = __ballot_sync(0xffffffffu, in);
+            if (in) idx[at + __popc(kept & below)] = j;
+            at += __popc(kept), ties += __popc(eq);
+        }
+    }
+    for (int i = want + threadIdx.x; i < A.keep; i += ST) idx[i] = n - A.keep + i;
+    __syncthreads();
+    // the totals, down in order: a run is read whole before it is written (in place no later run reads what it writes)
+    for (int i0 = 0; i0 < A.keep; i0 += ST) {
+        const int i = i0 + threadIdx.x;
+        const uint32_t v = i < A.keep ? bits(idx[i]) : 0u;
+        __syncthreads();
+        if (i < A.keep) tot_d[i] = v;
     }
 }
 
 constexpr int MT = 256;  // threads of a moving block
-constexpr int MC = 8;    // 16-byte pieces a thread holds
+constexpr int MC = 4;    // 16-byte pieces a thread holds of a run of rows
 
-// The kept rows of one (layer, kv head) of K (z = 0) or V (z = 1) moved in order. In place a row's destination is never
-// past its source, so a block that walks the rows in order, reads a run of them whole and writes it before it reads
-// the next never writes a row that it has still to read.
+// The kept rows of one (layer, kv head) of K or V in order, a run of rows at a time: the next run's pieces are asked for, this
+// run's have arrived in every thread, then this run is written. In place a row's destination is never past its source, so
+// a run that is written hits no row of a later run. More blocks share the work where heads and layers are few: in place
+// each takes a slice of every row's columns, else a range of the rows.
 __global__ void __launch_bounds__(MT) evict_move(const EvictArgs A) {
     pdl_launch_dependents();
     pdl_wait();
-    const int g = blockIdx.x, a = blockIdx.y, n = *A.n_seen;
-    const int kept = min(n, A.keep), per = A.D / 8;  // pieces of a row
-    const size_t at = (size_t)a * A.Hk + g;
-    const int* idx = A.idx + at * A.keep;
-    if (blockIdx.z == 2) {  // the totals
-        const float* src = A.totals + at * A.cap;
-        float* dst = A.totals_d + at * A.cap_d;
-        for (int j0 = 0; j0 < kept; j0 += MT) {
-            const int j = j0 + threadIdx.x;
-            const float v = j < kept ? src[idx[j]] : 0.f;
-            __syncthreads();
-            if (j < kept) dst[j] = v;
-            __syncthreads();
-        }
-        if (g == 0 && a == 0 && threadIdx.x == 0) *A.n_out = kept;
-        return;
-    }
-    const bf16* src = (blockIdx.z == 0 ? A.K : A.V) + (size_t)a * A.ls + (size_t)g * A.hs;
-    bf16* dst = (blockIdx.z == 0 ? A.Kd : A.Vd) + (size_t)a * A.ld + (size_t)g * A.hs;
-    const long long pieces = (long long)kept * per;
-    for (long long p0 = 0; p0 < pieces; p0 += MT * MC) {
+    const int g = blockIdx.x, a = blockIdx.y, kv = blockIdx.z & 1, part = blockIdx.z >> 1;
+    const int kept = min(*A.n_seen, A.keep);
+    if (kept < 0) return;  // refused
+    if (g == 0 && a == 0 && blockIdx.z == 0 && threadIdx.x == 0) *A.n_out = kept;
+    const int slices = A.in_place ? A.parts : 1, per = A.D / 8 / slices;  // pieces of a row's slice
+    const int span = A.in_place ? kept : (kept + A.parts - 1) / A.parts;
+    const int lo = A.in_place ? 0 : part * span, hi = min(kept, lo + span);
+    const int row = threadIdx.x / per, col = threadIdx.x - row * per, rows = MT / per;  // rows of a pass over the block's threads
+    const bool on = row < rows;
+    const int* idx = A.idx + ((size_t)a * A.Hk + g) * A.keep;
+    const size_t cols = (size_t)(A.in_place ? part * per : 0) + col;
+    const uint4* src = reinterpret_cast<const uint4*>((kv == 0 ? A.K : A.V) + (size_t)a * A.ls + (size_t)g * A.hs) + cols;
+    uint4* dst = reinterpret_cast<uint4*>((kv == 0 ? A.Kd : A.Vd) + (size_t)a * A.ld + (size_t)g * A.hs) + cols;
+    const size_t rs = (size_t)(A.rs / 8);
+    const int run = rows * MC;
+    auto from = [&](int i) {  // the cache row of kept row i, -1 past the end or outside the cache
+        if (!on || i >= hi) return -1;
+        int r = idx[i];
+        if (A.tbl != nullptr) r = A.tbl[r];
+        if (r >= 0 && r < A.cap) return r;
+        b2_fail(B2_ERR_DOMAIN);
+        return -1;
+    };
+    int ahead[MC];
+    uint4 next[MC];
+#pragma unroll
+    for (int c = 0; c < MC; ++c) ahead[c] = from(lo + c * rows + row);
+#pragma unroll
+    for (int c = 0; c < MC; ++c) next[c] = ahead[c] >= 0 ? src[ahead[c] * rs] : make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+    for (int c = 0; c < MC; ++c) ahead[c] = from(lo + run + c * rows + row);
+#pragma unroll 1
+    for (int i0 = lo; i0 < hi; i0 += run) {
         uint4 v[MC];
 #pragma unroll
-        for (int c = 0; c < MC; ++c) {
-            const long long p = p0 + c * MT + threadIdx.x;
-            if (p >= pieces) continue;
-            int r = idx[p / per];
-            if (A.tbl != nullptr) r = A.tbl[r];
-            if (r < 0 || r >= A.cap) {
-                b2_fail(B2_ERR_DOMAIN);
-                r = -1;
-            }
-            v[c] = r >= 0 ? reinterpret_cast<const uint4*>(src + (size_t)r * A.rs)[p % per] : make_uint4(0u, 0u, 0u, 0u);
+        for (int c = 0; c < MC; ++c) v[c] = next[c];
+#pragma unroll
+        for (int c = 0; c < MC; ++c) next[c] = ahead[c] >= 0 ? src[ahead[c] * rs] : make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+        for (int c = 0; c < MC; ++c) ahead[c] = from(i0 + 2 * run + c * rows + row);
+        if (A.in_place) {
+#pragma unroll
+            for (int c = 0; c < MC; ++c) asm volatile("" ::"r"(v[c].x), "r"(v[c].y), "r"(v[c].z), "r"(v[c].w));  // they are here
+            __syncthreads();
         }
-        __syncthreads();
 #pragma unroll
         for (int c = 0; c < MC; ++c) {
-            const long long p = p0 + c * MT + threadIdx.x;
-            if (p >= pieces) continue;
-            int r = (int)(p / per);
-            if (A.tbl_d != nullptr) r = A.tbl_d[r];
+            const int i = i0 + c * rows + row;
+            if (!on || i >= hi) continue;
+            const int r = A.tbl_d != nullptr ? A.tbl_d[i] : i;
             if (r < 0 || r >= A.cap_d) b2_fail(B2_ERR_DOMAIN);
-            else reinterpret_cast<uint4*>(dst + (size_t)r * A.rs)[p % per] = v[c];
+            else dst[r * rs] = v[c];
         }
-        __syncthreads();
     }
 }
+
+// a launch that may start while the one before it drains (bit 3 of the `pdl` tunable)
+constexpr int KIND = 8;
 
 }  // namespace
 
@@ -188,8 +234,8 @@ extern "C" int btb_b200_kv_evict(const void* K, const void* V, const void* total
                                  long long hs, long long rs, int cap, int cap_d, int keep, int recent, const void* tbl,
                                  const void* tbl_d, void* workspace, void* stream) {
     if (!K || !V || !totals || !n0p || !Kd || !Vd || !totals_d || !n_out || !idx || !workspace) return B2_ERR_NULL;
-    if (layers <= 0 || layers > 65535 || Hk <= 0 || D <= 0 || (D & 7) || cap <= 0 || cap_d <= 0 || keep <= 0 || keep > cap_d ||
-        recent < 0 || recent > keep || hs < D || rs < D || (hs & 7) || (rs & 7) || (ls & 7) || (ld & 7))
+    if (layers <= 0 || layers > 65535 || Hk <= 0 || D <= 0 || D > 8 * MT || (D & 7) || cap <= 0 || cap_d <= 0 || keep <= 0 ||
+        keep > cap_d || recent < 0 || recent > keep || hs < D || rs < D || (hs & 7) || (rs & 7) || (ls & 7) || (ld & 7))
         return B2_ERR_DOMAIN;
     if ((reinterpret_cast<uintptr_t>(K) | reinterpret_cast<uintptr_t>(V) | reinterpret_cast<uintptr_t>(Kd) |
          reinterpret_cast<uintptr_t>(Vd) | reinterpret_cast<uintptr_t>(workspace)) & 15)
@@ -200,8 +246,21 @@ extern "C" int btb_b200_kv_evict(const void* K, const void* V, const void* total
     EvictArgs a{static_cast<const bf16*>(K), static_cast<const bf16*>(V), static_cast<const float*>(totals),
                 static_cast<const int*>(n0p), static_cast<bf16*>(Kd), static_cast<bf16*>(Vd), static_cast<float*>(totals_d),
                 static_cast<int*>(n_out), static_cast<int*>(idx), static_cast<const int*>(tbl), static_cast<const int*>(tbl_d),
-                static_cast<int*>(workspace), ls, ld, hs, rs, layers, Hk, D, cap, cap_d, keep, recent};
+                static_cast<int*>(workspace), ls, ld, hs, rs, layers, Hk, D, cap, cap_d, keep, recent, 0, 1, in_k};
+    a.held = cap <= 48 * 1024;
+    // blocks for every SM several times over: slices of a row's columns of at least 64 bytes in place, else ranges of at least
+    // two runs of rows
+    const long long heads = 2LL * layers * Hk, fill = 8LL * b2_sm_count();
+    if (a.in_place) {
+        while (a.parts < 4 && heads * a.parts < fill / 2 && D % (a.parts * 2 * 32) == 0) a.parts *= 2;
+    } else {
+        const int run = MT / (D / 8) * MC;
+        while (a.parts < 256 && heads * a.parts < fill && (long long)a.parts * 4 * run <= keep) a.parts *= 2;
+    }
+    static bool allowed[64];
+    if (const int rc = b2_allow_smem(reinterpret_cast<const void*>(evict_pick), allowed)) return rc;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (const int rc = b2_launch(reinterpret_cast<const void*>(evict_pick), dim3(Hk, layers), dim3(ST), 0, s, a)) return rc;
-    return b2_launch(reinterpret_cast<const void*>(evict_move), dim3(Hk, layers, 3), dim3(MT), 0, s, a);
+    if (const int rc = b2_launch(reinterpret_cast<const void*>(evict_pick), dim3(Hk, layers), dim3(ST), a.held ? (size_t)cap * 4 : 0, s, a, KIND))
+        return rc;
+    return b2_launch(reinterpret_cast<const void*>(evict_move), dim3(Hk, layers, 2 * a.parts), dim3(MT), 0, s, a, KIND);
 }

@@ -506,7 +506,7 @@ def test_evict_refuses_a_count_outside_the_cache_and_a_bad_map():
     K0, V0, t0 = K.clone(), V.clone(), t.clone()
     for n0 in (101, -1, 1 << 30, -(1 << 31)):
         _, n_out = evict(K, V, t, n0, 50, 10)
-        assert torch.equal(K, K0) and torch.equal(V, V0) and torch.equal(t, t0)
+        assert torch.equal(K, K0) and torch.equal(V, V0) and torch.equal(t, t0) and int(n_out) == -7
         assert capi.status() == capi.ERR_DOMAIN
     for v in (-1, 100, 1 << 30):
         tbl = torch.arange(100, dtype=torch.int32, device=DEV)
