@@ -28,6 +28,7 @@ struct LongArgs {
     float* lse;          // [T, Hq] log2 of a row's denominator
     float* own;          // [T, Hq, 32] the scores of the pass's own rows in log2 units, -inf where not seen
     float* scores;       // [Hq, T, score_n] the scores of all keys in log2 units (passes of few rows), or null
+    int4* info;          // [T] two words a row: where its states lie
     float2* part_ml;     // a part's rows, then the units': maximum and sum ...
     float* part_o;       // ... and output [., D], not yet divided
     long long unit_row;  // the units' first row: unit u of kv head g at unit_row + (g * units + u) * G
@@ -39,23 +40,25 @@ struct LongArgs {
 
 // ---- the pass's work, from what stands on the card ------------------------------------------------------------------
 // The prefixes: per kv head an item for each prefix that rows share, its queries all of those rows', its keys cut into
-// tiles of 64. The tiles of all heads in one line are cut evenly over the CTAs; a CTA's stretch of an item is a part, whose
-// state (maximum, sum, output row) the joining kernel folds with the others'. Part (CTA c, item i) keeps its rows at
+// tiles of 64. The tiles of all heads lie in one line, with a gap of GAP tiles' worth of time behind each item (what it costs
+// a CTA to end one and begin the next), which is cut evenly over the CTAs; a CTA's stretch of an item is a part, whose state
+// (maximum, sum, output row) the joining kernel folds with the others'. Part (CTA c, item i) keeps its rows at
 // c * T G + the rows of all items before i, which no two parts share.
 // A row's own keys (its steps in the rows layout, its path in a chain or tree pass) are no one else's: units of up to
 // `chunk` keys of one (row, kv head), a warp each, beside the tiles. A one-row pass's own key joins its prefix.
 constexpr int KT = 64;         // keys a tile
+constexpr int GAP = 4;
 constexpr int CTAS_MAX = 160;  // CTAs of the tile kernel at most
 constexpr int OWN_WARPS = 2;   // warps of a CTA that take units (two more would leave all of them 128 registers)
 
 struct Plan {
     int mask[32];                             // item of lane l's prefix: its rows (0: no item)
     int p_start[32], p_count[32];             // ... its first key (cache row, or logical row of a chain or tree pass) and keys
-    int p_tiles[32], p_tile0[32], p_row0[32]; // ... tiles, tiles and partial rows before it (within a kv head)
+    int p_tiles[32], p_at[32], p_row0[32];    // ... tiles, its first one's place in a kv head's line, partial rows before it
     int order[32];                            // ... its rows, from p_row0 / G on
     int lead[32];                             // row t's prefix item, -1: padding or refused
     int own[32], own_n[32], unit0[32];        // its own keys: the first's cache row (rows layout), how many; units before it
-    int W, tiles, rows, units, chunk, n0;     // ... and the kv head's tiles, partial rows and units
+    int W, line, rows, units, chunk, n0;      // ... and a kv head's length of line, partial rows and units
 };
 
 __device__ __forceinline__ int warp_excl(int v, int lane, int& total) {
@@ -72,8 +75,9 @@ __device__ __forceinline__ int warp_excl(int v, int lane, int& total) {
 // units of a (row, kv head) at most: enough for every warp where rows and heads are few
 __host__ __device__ __forceinline__ int units_max(int T, int Hk) { return max(16, min(64, 1024 / (T * Hk))); }
 
-// one warp fills `P`; `tell`: this block records a refused layout
-__device__ __forceinline__ void make_plan(const LongArgs& A, int G, Plan& P, bool tell) {
+// one warp fills `P`; `tell`: this block records a refused layout and the rows' places for the joining kernel
+template <int G>
+__device__ __forceinline__ void make_plan(const LongArgs& A, Plan& P, bool tell) {
     const int t = threadIdx.x & 31;
     int mask = 0, start = 0, count = 0, lead = -1, own = 0, own_n = 0, W = 0, n0 = 0;
     if (A.rw == nullptr) {
@@ -120,56 +124,66 @@ __device__ __forceinline__ void make_plan(const LongArgs& A, int G, Plan& P, boo
         }
     }
     const int p_tiles = mask ? (count + KT - 1) / KT : 0;
-    int pt, pr, keys, units;
-    const int p_tile0 = warp_excl(p_tiles, t, pt), p_row0 = warp_excl(p_tiles ? __popc(mask) * G : 0, t, pr);
+    int line, pr, units;
+    const int p_at = warp_excl(p_tiles ? p_tiles + GAP : 0, t, line), p_row0 = warp_excl(p_tiles ? __popc(mask) * G : 0, t, pr);
     // units of about a warp's fair share of the own keys, a multiple of 32, no row in more of them than its room allows
-    (void)warp_excl(min(own_n, 1 << 20), t, keys);
+    const int keys = __reduce_add_sync(0xffffffffu, min(own_n, 1 << 20));
     int chunk = (int)(((long long)keys * A.Hk + A.ctas * OWN_WARPS - 1) / (A.ctas * OWN_WARPS));
     const int most = __reduce_max_sync(0xffffffffu, own_n), room = units_max(A.T, A.Hk);
     chunk = (max(chunk, (most + room - 1) / room) + 31) & ~31;
     const int unit0 = warp_excl(own_n > 0 ? (own_n + chunk - 1) / chunk : 0, t, units);
-    P.mask[t] = mask, P.p_start[t] = start, P.p_count[t] = count, P.p_tiles[t] = p_tiles, P.p_tile0[t] = p_tile0, P.p_row0[t] = p_row0;
+    P.mask[t] = mask, P.p_start[t] = start, P.p_count[t] = count, P.p_tiles[t] = p_tiles, P.p_at[t] = p_at, P.p_row0[t] = p_row0;
     P.lead[t] = lead, P.own[t] = own, P.own_n[t] = own_n, P.unit0[t] = unit0;
     const int src = lead < 0 ? 0 : lead;
-    const int its = __shfl_sync(0xffffffffu, mask, src), before = __shfl_sync(0xffffffffu, p_row0, src), some = __shfl_sync(0xffffffffu, p_tiles, src);
-    if (lead >= 0 && some > 0) P.order[before / G + __popc(its & ((1u << t) - 1u))] = t;
-    if (t == 0) P.W = W, P.tiles = pt, P.rows = pr, P.units = units, P.chunk = chunk, P.n0 = n0;
+    const int its = __shfl_sync(0xffffffffu, mask, src), before = __shfl_sync(0xffffffffu, p_row0, src);
+    const int some = __shfl_sync(0xffffffffu, p_tiles, src), at = __shfl_sync(0xffffffffu, p_at, src);
+    const int below = __popc(its & ((1u << t) - 1u));  // the row's place among its prefix's
+    if (lead >= 0 && some > 0) P.order[before / G + below] = t;
+    if (tell && t < A.T) {  // for the joining kernel: where the row's states lie (none: padding, or refused)
+        A.info[2 * t] = make_int4(at, lead < 0 ? 0 : some, before + below * G, own_n > 0 ? (own_n + chunk - 1) / chunk : 0);
+        A.info[2 * t + 1] = make_int4(unit0, line, pr, units);
+    }
+    if (t == 0) P.W = W, P.line = line, P.rows = pr, P.units = units, P.chunk = chunk, P.n0 = n0;
     __syncwarp();
 }
 
-// the even cut of `tiles` tiles over the CTAs; only as many of them have any as there are tiles, so that no stretch between
-// two others is empty
+// the even cut of the heads' line over the CTAs; no more of them than it is long, so that no stretch between two others is
+// empty
 struct Cut {
-    int per, more;  // the first `more` CTAs have per + 1 tiles
-    __device__ __forceinline__ Cut(int tiles, int ctas) : per(tiles / ctas), more(tiles - tiles / ctas * ctas) {}
+    int per, more;  // the first `more` CTAs' stretches are per + 1 long
+    __device__ __forceinline__ Cut(int line, int ctas) : per(line / ctas), more(line - line / ctas * ctas) {}
     __device__ __forceinline__ int first(int c) const { return c * per + min(c, more); }
-    __device__ __forceinline__ int cta_of(int tile) const {
+    __device__ __forceinline__ int cta_of(int place) const {
         const int big = more * (per + 1);
-        return tile < big ? tile / (per + 1) : more + (tile - big) / per;
+        return place < big ? place / (per + 1) : more + (place - big) / per;
     }
 };
 
 // a CTA's stretch of one item
 struct Part {
     int head, start, keys, tiles, rows, order;  // `keys`: of these tiles (the last may be partly filled)
-    int end;                                    // the first tile past it
+    int end;                                    // the place behind it
     long long row0;                             // its first partial row
 };
-// the part that begins at tile `at` of a CTA whose stretch ends at `stop` (every lane of a warp asks alike)
-__device__ __noinline__ Part part_at(const Plan& P, int span, int G, int at, int stop, int cta) {
+// the first part at or behind place `at` of a CTA whose stretch ends at `stop`; tiles 0: none (a warp's lanes ask alike)
+template <int G>
+__device__ __noinline__ Part part_at(const Plan& P, int span, int at, int stop, int cta) {
     const int lane = threadIdx.x & 31;
     Part p;
-    p.head = at / P.tiles;
-    const int in = at - p.head * P.tiles;
-    const int l = __ffs(__ballot_sync(0xffffffffu, in >= P.p_tile0[lane] && in < P.p_tile0[lane] + P.p_tiles[lane])) - 1;
-    const int skip = in - P.p_tile0[l];
-    p.tiles = min(P.p_tiles[l] - skip, stop - at);
+    p.head = at / P.line;
+    int in = at - p.head * P.line;
+    const int first = P.p_at[lane], tiles = P.p_tiles[lane];
+    const unsigned here = __ballot_sync(0xffffffffu, tiles > 0 && first + tiles > in);  // items not yet behind
+    if (here == 0) ++p.head, in = 0;                                                     // (in the head's last gap)
+    const unsigned any = here != 0 ? here : __ballot_sync(0xffffffffu, tiles > 0);
+    const int l = __ffs(any) - 1, skip = max(in - P.p_at[l], 0), place = p.head * P.line + P.p_at[l] + skip;
+    p.tiles = max(min(P.p_tiles[l] - skip, stop - place), 0);
     p.start = P.p_start[l] + skip * KT;
     p.keys = min(p.tiles * KT, P.p_count[l] - skip * KT);
     p.rows = __popc(P.mask[l]) * G;
     p.order = P.p_row0[l] / G;
     p.row0 = (long long)cta * span + (long long)p.head * P.rows + P.p_row0[l];
-    p.end = at + p.tiles;
+    p.end = place + p.tiles;
     return p;
 }
 
@@ -318,6 +332,15 @@ __device__ __forceinline__ bool wait_or_fail(uint64_t* bar, uint32_t parity, Til
     return __all_sync(0xffffffffu, mbar_try_wait(b, parity)) || wait_long(b, parity, sy);
 }
 
+// the place of the n-th (from 0) set bit
+__device__ __forceinline__ int bit_place(unsigned set, int n) {
+    int at = 0;
+#pragma unroll
+    for (int s = 16; s > 0; s >>= 1)
+        if (__popc(set & ((1u << (at + s)) - 1u)) <= n) at += s;
+    return at;
+}
+
 // a warp's units: every `stride`-th from `first` on. A lane a key for the scores and D / 32 dims for the output, a running
 // maximum and sum over 32 keys at a time; keys outside are never read.
 template <int D, int G>
@@ -346,7 +369,7 @@ __device__ __forceinline__ void own_units(const LongArgs& A, const Plan& P, int 
                 if (A.rw != nullptr) {
                     row = own + (i0 + j0 + lane) * P.W;
                 } else {
-                    row = P.n0 + (int)__fns((unsigned)own, 0, j0 + lane + 1);
+                    row = P.n0 + bit_place((unsigned)own, j0 + lane);
                     if (A.tbl != nullptr) row = A.tbl[row];
                     if (row < 0 || row >= A.cap) {
                         b2_fail(B2_ERR_DOMAIN);
@@ -467,9 +490,9 @@ __global__ void __launch_bounds__(TW * 32, 1)
     // the kernels before are through; only now may the joining kernel start, which reads what they left before it waits
     pdl_wait();
     pdl_launch_dependents();
-    if (warp == 0) make_plan(A, G, plan, blockIdx.x == 0);
+    if (warp == 0) make_plan<G>(A, plan, blockIdx.x == 0);
     __syncthreads();
-    const Cut cut(plan.tiles * A.Hk, gridDim.x);
+    const Cut cut(plan.line * A.Hk, gridDim.x);
     const int begin = cut.first(blockIdx.x);
     const int stop = sq & 1023 ? begin : cut.first(blockIdx.x + 1);  // (the tiles leave no room to align them here)
     tm_after();
@@ -485,24 +508,29 @@ __global__ void __launch_bounds__(TW * 32, 1)
         uint32_t stph = 0, nph = 0;
         bool ok = true;
         for (int at = begin; at < stop && ok;) {
-            const Part p = part_at(plan, A.T * G, G, at, stop, blockIdx.x);
+            const Part p = part_at<G>(plan, A.T * G, at, stop, blockIdx.x);
+            if (p.tiles == 0) break;
             at = p.end;
             const bool two = p.rows > 128;
             {   // the part's queries into shared memory as the MMA reads them: 16-byte piece c of row r at c ^ (r & 7)
                 const uint32_t flip = A.scale < 0.f ? 0x80008000u : 0u;
-#pragma unroll 1
-                for (int rt = 0; rt < (two ? 2 : 1); ++rt) {
+                uint4 v[2][D / 16];
+#pragma unroll
+                for (int rt = 0; rt < 2; ++rt) {
                     const int r = rt * 128 + row;
                     const int t = r < p.rows ? plan.order[p.order + r / G] : 0;
                     const uint4* src = reinterpret_cast<const uint4*>(A.q + ((size_t)t * A.Hq + p.head * G + r % G) * D) + wg * (D / 16);
-                    uint4 v[D / 16];
 #pragma unroll
-                    for (int c = 0; c < D / 16; ++c) v[c] = r < p.rows ? src[c] : make_uint4(0u, 0u, 0u, 0u);
+                    for (int c = 0; c < D / 16; ++c) v[rt][c] = r < p.rows ? src[c] : make_uint4(0u, 0u, 0u, 0u);
+                }
+#pragma unroll
+                for (int rt = 0; rt < 2; ++rt) {
+                    if (rt == 1 && !two) break;
 #pragma unroll
                     for (int c = 0; c < D / 16; ++c) {
-                        v[c].x ^= flip, v[c].y ^= flip, v[c].z ^= flip, v[c].w ^= flip;
+                        v[rt][c].x ^= flip, v[rt][c].y ^= flip, v[rt][c].z ^= flip, v[rt][c].w ^= flip;
                         const int piece = wg * (D / 16) + c;
-                        *reinterpret_cast<uint4*>(smem + rt * QTILE + (piece >> 3) * QHALF + row * 128 + (((piece & 7) ^ (row & 7)) << 4)) = v[c];
+                        *reinterpret_cast<uint4*>(smem + rt * QTILE + (piece >> 3) * QHALF + row * 128 + (((piece & 7) ^ (row & 7)) << 4)) = v[rt][c];
                     }
                 }
                 fence_proxy_async();
@@ -651,7 +679,8 @@ __global__ void __launch_bounds__(TW * 32, 1)
         uint32_t ph = 1;                // (the first round finds the stages empty)
         bool ok = true;
         for (int at = begin; at < stop && ok;) {
-            const Part p = part_at(plan, A.T * G, G, at, stop, blockIdx.x);
+            const Part p = part_at<G>(plan, A.T * G, at, stop, blockIdx.x);
+            if (p.tiles == 0) break;
             at = p.end;
             const int x = p.head * X.col_mul, y0 = p.head * X.row_mul;
 #pragma unroll 1
@@ -709,7 +738,8 @@ __global__ void __launch_bounds__(TW * 32, 1)
         uint32_t kph = 0, vph = 0, qph = 0, scount0 = 0, scount1 = 0, pcount0 = 0, pcount1 = 0;
         bool ok = true;
         for (int at = begin; at < stop && ok;) {
-            const Part p = part_at(plan, A.T * G, G, at, stop, blockIdx.x);
+            const Part p = part_at<G>(plan, A.T * G, at, stop, blockIdx.x);
+            if (__shfl_sync(0xffffffffu, p.tiles, 0) == 0) break;
             at = __shfl_sync(0xffffffffu, p.end, 0);
             // job j: tile j for warpgroup j & 1, or both warpgroups' halves of tile j / 2; scores run four jobs ahead
             const int nrt = __shfl_sync(0xffffffffu, p.rows, 0) > 128 ? 2 : 1, jobs = __shfl_sync(0xffffffffu, p.tiles, 0) * nrt;
@@ -770,19 +800,19 @@ constexpr int KEEP_ROWS = 16;              // a kv head's queries (T G) up to wh
 struct States {
     long long p_row, u_row;
     int np, n, step, G;
-    __device__ __forceinline__ States(const LongArgs& A, const Plan& P, int t, int g, int G_) : G(G_) {
-        const int lead = P.lead[t], tile = g * P.tiles + P.p_tile0[lead];
-        const Cut cut(P.tiles * A.Hk, A.ctas);
+    __device__ __forceinline__ States(const LongArgs& A, int t, int g, int G_) : G(G_) {
+        const int4 a = __ldcg(A.info + 2 * t), b = __ldcg(A.info + 2 * t + 1);  // place, tiles, row, units; unit, line, rows, units
+        const int place = g * b.y + a.x;
         int c = 0;
         np = 0, step = A.T * G;
-        if (P.p_tiles[lead] > 0) {
-            c = cut.cta_of(tile);
-            np = cut.cta_of(tile + P.p_tiles[lead] - 1) - c + 1;
+        if (a.y > 0) {
+            const Cut cut(b.y * A.Hk, A.ctas);
+            c = cut.cta_of(place);
+            np = cut.cta_of(place + a.y - 1) - c + 1;
         }
-        const int below = __popc(P.mask[lead] & ((1u << t) - 1u));  // the row's place among its prefix's
-        p_row = (long long)c * step + (long long)g * P.rows + P.p_row0[lead] + below * G;
-        u_row = A.unit_row + ((long long)g * P.units + P.unit0[t]) * G;
-        n = np + (P.own_n[t] > 0 ? (P.own_n[t] + P.chunk - 1) / P.chunk : 0);
+        p_row = (long long)c * step + (long long)g * b.z + a.z;
+        u_row = A.unit_row + ((long long)g * b.w + b.x) * G;
+        n = np + a.w;
     }
     __device__ __forceinline__ long long at(int k) const { return k < np ? p_row + (long long)k * step : u_row + (long long)(k - np) * G; }
 };
@@ -792,15 +822,15 @@ __device__ __forceinline__ void row_stats(const LongArgs& A, const States& S, in
     const int lane = threadIdx.x & 31;
     const float sink = A.sinks != nullptr ? __fmul_rn(A.sinks[head], LOG2E) : NEG_INF;
     M = sink;
-    const float2 first = lane < S.n ? A.part_ml[S.at(lane) + hh] : make_float2(NEG_INF, 0.f);
+    const float2 first = lane < S.n ? __ldcg(A.part_ml + S.at(lane) + hh) : make_float2(NEG_INF, 0.f);
     M = fmaxf(M, first.x);
-    for (int k = lane + 32; k < S.n; k += 32) M = fmaxf(M, A.part_ml[S.at(k) + hh].x);
+    for (int k = lane + 32; k < S.n; k += 32) M = fmaxf(M, __ldcg(A.part_ml + S.at(k) + hh).x);
 #pragma unroll
     for (int k = 16; k > 0; k >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, k));
     const float sub = M == NEG_INF ? 0.f : M;
     L = 0.f;
     for (int k = lane; k < S.n; k += 32) {
-        const float2 ml = k == lane ? first : A.part_ml[S.at(k) + hh];
+        const float2 ml = k == lane ? first : __ldcg(A.part_ml + S.at(k) + hh);
         const float f = ml.x == NEG_INF ? 0.f : ex2(ml.x - sub);
         L += f * ml.y;
         if (fac != nullptr) fac[k] = f;
@@ -816,38 +846,44 @@ __device__ __forceinline__ void row_stats(const LongArgs& A, const States& S, in
 template <int D, int G>
 __global__ void __launch_bounds__(JT) long_join(const LongArgs A, int weight_blocks) {
     constexpr int E = D / 32, WH = JW / G;  // warps a query head
-    __shared__ Plan plan;
     __shared__ float fac[JW][STATES_MAX];
     __shared__ __align__(16) float part[JW][D];
     __shared__ float s_lse[KEEP_ROWS];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     pdl_launch_dependents();
-    if (warp == 0) make_plan(A, G, plan, false);
-    __syncthreads();
+    pdl_wait();
     if ((int)blockIdx.x < A.T * A.Hk) {
         const int t = blockIdx.x / A.Hk, g = blockIdx.x - t * A.Hk, hh = warp / WH, sub = warp - hh * WH, head = g * G + hh;
-        if (plan.lead[t] < 0) {  // padding, or refused
-            pdl_wait();
-            return;
-        }
-        const States S(A, plan, t, g, G);
-        pdl_wait();
+        const States S(A, t, g, G);
+        if (S.n == 0) return;  // padding, or refused
         float M, L;
         row_stats(A, S, head, hh, M, L, fac[warp]);
         __syncwarp();
         float o[E];
 #pragma unroll
         for (int e = 0; e < E; ++e) o[e] = 0.f;
-#pragma unroll 4
-        for (int k = sub; k < S.n; k += WH) {
-            const float f = fac[warp][k];
-            const float* src = A.part_o + (size_t)(S.at(k) + hh) * D + lane * E;
-            if (E == 4) {
-                const float4 v = *reinterpret_cast<const float4*>(src);
-                o[0] = fmaf(f, v.x, o[0]), o[1] = fmaf(f, v.y, o[1]), o[E - 2] = fmaf(f, v.z, o[E - 2]), o[E - 1] = fmaf(f, v.w, o[E - 1]);
-            } else {
-                const float2 v = *reinterpret_cast<const float2*>(src);
-                o[0] = fmaf(f, v.x, o[0]), o[E - 1] = fmaf(f, v.y, o[E - 1]);
+        constexpr int B = 8;  // states in flight
+#pragma unroll 1
+        for (int k0 = sub; k0 < S.n; k0 += B * WH) {
+            float v[B][E];
+#pragma unroll
+            for (int j = 0; j < B; ++j) {
+                const int k = min(k0 + j * WH, S.n - 1);
+                const float* src = A.part_o + (size_t)(S.at(k) + hh) * D + lane * E;
+                if (E == 4) {
+                    const float4 x = __ldcg(reinterpret_cast<const float4*>(src));
+                    v[j][0] = x.x, v[j][1] = x.y, v[j][E - 2] = x.z, v[j][E - 1] = x.w;
+                } else {
+                    const float2 x = __ldcg(reinterpret_cast<const float2*>(src));
+                    v[j][0] = x.x, v[j][E - 1] = x.y;
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < B; ++j) {
+                if (k0 + j * WH >= S.n) break;
+                const float f = fac[warp][k0 + j * WH];
+#pragma unroll
+                for (int e = 0; e < E; ++e) o[e] = fmaf(f, v[j][e], o[e]);
             }
         }
         if (WH > 1) {
@@ -870,13 +906,13 @@ __global__ void __launch_bounds__(JT) long_join(const LongArgs A, int weight_blo
         return;
     }
     // ---- the weights ------------------------------------------------------------------------------------------------------
-    const int b = blockIdx.x - A.T * A.Hk, g = b / weight_blocks, n = plan.n0 + (A.T == 1);  // keys whose scores were kept
+    const int b = blockIdx.x - A.T * A.Hk, g = b / weight_blocks, n0 = __ldcg(A.n0p);
+    const int n = n0 < 0 || n0 > A.cap - A.T ? -1 : n0 + (A.T == 1);  // keys whose scores were kept; -1: refused
     int j = (b - g * weight_blocks) * JT + threadIdx.x;
-    pdl_wait();
-    if (plan.lead[0] < 0 || (j - (int)threadIdx.x >= n && b != g * weight_blocks)) return;
+    if (n < 0 || (j - (int)threadIdx.x >= n && b != g * weight_blocks)) return;
     for (int r = warp; r < A.T * G; r += JW) {
         const int t = r / G, hh = r - t * G;
-        const States S(A, plan, t, g, G);
+        const States S(A, t, g, G);
         float M, L;
         row_stats(A, S, g * G + hh, hh, M, L, nullptr);
         if (lane == 0) s_lse[r] = M + log2f(L);
@@ -887,13 +923,13 @@ __global__ void __launch_bounds__(JT) long_join(const LongArgs A, int weight_blo
         float a = 0.f;
         for (int r = 0; r < A.T * G; ++r)
             a += ex2(A.own[((size_t)(r / G) * A.Hq + g * G + r % G) * 32 + threadIdx.x] - s_lse[r]);
-        tot[plan.n0 + threadIdx.x] = a;
+        tot[n0 + threadIdx.x] = a;
     }
     for (; j < n; j += weight_blocks * JT) {
         float a = 0.f;
 #pragma unroll 8
         for (int r = 0; r < A.T * G; ++r) a += ex2(A.scores[((size_t)g * A.T * G + r) * A.score_n + j] - s_lse[r]);
-        tot[j] = j < plan.n0 ? tot[j] + a : a;
+        tot[j] = j < n0 ? tot[j] + a : a;
     }
 }
 
@@ -1082,6 +1118,7 @@ int long_ctas() { return min(b2_sm_count(), CTAS_MAX); }
 // rows of the parts at most: every CTA's stretch moves on by one item's rows, every kv head by its items'
 size_t part_rows(int T, int Hq) { return (size_t)long_ctas() * T * Hq + (size_t)T * Hq; }
 size_t state_rows(int T, int Hq, int Hk) { return part_rows(T, Hq) + (size_t)T * Hq * units_max(T, Hk); }
+constexpr size_t INFO_BYTES = TMAX * 2 * sizeof(int4);
 long long score_stride(int cap) { return ((long long)cap + KT - 1) / KT * KT; }
 bool keeps_scores(int T, int Hq, int Hk) { return T * (Hq / Hk) <= KEEP_ROWS; }
 
@@ -1143,13 +1180,15 @@ int check_cache(const void* q, const void* K, const void* V, const void* out, in
 }  // namespace
 
 extern "C" size_t btb_b200_attn_shared_workspace_bytes(int T, int Hq, int Hk, int D) {
-    return shape_ok(T, Hq, Hk, D) ? state_rows(T, Hq, Hk) * (D * 4 + 8) : 0;
+    return shape_ok(T, Hq, Hk, D) ? state_rows(T, Hq, Hk) * (D * 4 + 8) + INFO_BYTES : 0;
 }
 
 // the states' place in a workspace; returns what lies behind it
 static float* take_states(LongArgs& a, void* workspace, int D) {
     const size_t rows = state_rows(a.T, a.Hq, a.Hk);
-    a.part_o = static_cast<float*>(workspace), a.part_ml = reinterpret_cast<float2*>(a.part_o + rows * D);
+    a.info = static_cast<int4*>(workspace);
+    a.part_o = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + INFO_BYTES);
+    a.part_ml = reinterpret_cast<float2*>(a.part_o + rows * D);
     a.unit_row = (long long)part_rows(a.T, a.Hq);
     return reinterpret_cast<float*>(a.part_ml + rows);
 }
@@ -1169,7 +1208,7 @@ extern "C" int btb_b200_attn_shared(const void* q, const void* K, const void* V,
 
 extern "C" size_t btb_b200_attn_scored_workspace_bytes(int T, int Hq, int Hk, int D, int cap) {
     if (!shape_ok(T, Hq, Hk, D) || cap <= 0) return 0;
-    size_t n = state_rows(T, Hq, Hk) * (D * 4 + 8) + (size_t)T * Hq * 33 * 4;
+    size_t n = INFO_BYTES + state_rows(T, Hq, Hk) * (D * 4 + 8) + (size_t)T * Hq * 33 * 4;
     if (keeps_scores(T, Hq, Hk)) n = ((n + 15) & ~(size_t)15) + (size_t)T * Hq * score_stride(cap) * 4;
     return n;
 }
