@@ -341,114 +341,161 @@ __device__ __forceinline__ int bit_place(unsigned set, int n) {
     return at;
 }
 
-// a warp's units: every `stride`-th from `first` on. A lane a key for the scores and D / 32 dims for the output, a running
-// maximum and sum over 32 keys at a time; keys outside are never read.
+__device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t turned(uint32_t v) {  // an 8 x 8 matrix of 16-bit values, two of a row a lane, transposed
+    uint32_t w;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(w) : "r"(v));
+    return w;
+}
+
+// a warp's units: every `stride`-th from `first` on, 32 keys at a time with a running maximum and sum. So few queries (a kv
+// head's of one row) on keys nobody shares want few instructions and early loads, not tiles: the products are warp MMAs
+// straight from registers. S (16 keys x 8 heads) takes 16 bytes of a key's row a lane: the lane's eight dims stand for the
+// products' k in an order of our own, the same for keys and queries. O (heads x dims) takes the weights and the values each
+// turned by movmatrix, 16 bytes of a value's row a lane. (As f32 chains, a lane a key, the units ended 4 us after the tiles of
+// 8 rows of 256 steps over a 2048-row prefix and 20 us after those of 32 rows of 128 steps over 32768: 23 and 83 us a call
+// where these take 17 and 62.) Lane 4 y + x: keys y, y + 8, ..; heads 2 x, 2 x + 1 of the
+// scores; head y and dims 32 c + 8 x .. + 7 of the output. Keys outside are never read.
 template <int D, int G>
 __device__ __forceinline__ void own_units(const LongArgs& A, const Plan& P, int first, int stride) {
-    constexpr int E = D / 32, VB = 16;
-    const int lane = threadIdx.x & 31;
+    constexpr int C = D / 32;
+    const int lane = threadIdx.x & 31, x = lane & 3, y = lane >> 2;
     const float scale2 = __fmul_rn(A.scale, LOG2E);
     const long long all = (long long)P.units * A.Hk;
     for (long long u = first; u < all; u += stride) {
         const int g = (int)(u / P.units), in = (int)(u - (long long)g * P.units);
         const int t = 31 - __clz(__ballot_sync(0xffffffffu, P.own_n[lane] > 0 && P.unit0[lane] <= in));
         const int i0 = (in - P.unit0[t]) * P.chunk, n = min(P.chunk, P.own_n[t] - i0), own = P.own[t];
-        const bf16* Kg = A.K + (size_t)g * A.hs;
-        const bf16* Vg = A.V + (size_t)g * A.hs;
-        const uint4* q = reinterpret_cast<const uint4*>(A.q + ((size_t)t * A.Hq + g * G) * D);
-        float m[G], l[G], o[G][E];
+        const bf16* Kg = A.K + (size_t)g * A.hs + x * 8;
+        const bf16* Vg = A.V + (size_t)g * A.hs + x * 8;
+        float* scores = A.own != nullptr ? A.own + ((size_t)t * A.Hq + g * G) * 32 : nullptr;
+        uint4 q[C];
 #pragma unroll
-        for (int hh = 0; hh < G; ++hh) {
-            m[hh] = NEG_INF, l[hh] = 0.f;
-#pragma unroll
-            for (int e = 0; e < E; ++e) o[hh][e] = 0.f;
+        for (int c = 0; c < C; ++c)
+            q[c] = y < G ? __ldg(reinterpret_cast<const uint4*>(A.q + ((size_t)t * A.Hq + g * G + y) * D + c * 32 + x * 8)) : make_uint4(0u, 0u, 0u, 0u);
+        if (scores != nullptr) {
+            for (int h = 0; h < G; ++h) scores[h * 32 + lane] = NEG_INF;
+            __syncwarp();
         }
-        for (int j0 = 0; j0 < n; j0 += 32) {
-            int row = -1;
-            if (j0 + lane < n) {
-                if (A.rw != nullptr) {
-                    row = own + (i0 + j0 + lane) * P.W;
-                } else {
-                    row = P.n0 + bit_place((unsigned)own, j0 + lane);
-                    if (A.tbl != nullptr) row = A.tbl[row];
-                    if (row < 0 || row >= A.cap) {
-                        b2_fail(B2_ERR_DOMAIN);
-                        row = -1;
-                    }
-                }
-            }
-            float s[G];
+        float m[2] = {NEG_INF, NEG_INF}, l[2] = {0.f, 0.f}, o[C][4][2];
 #pragma unroll
-            for (int hh = 0; hh < G; ++hh) s[hh] = 0.f;
-            const uint4* kr = reinterpret_cast<const uint4*>(Kg + (size_t)max(row, 0) * A.rs);
+        for (int c = 0; c < C; ++c)
 #pragma unroll
-            for (int c0 = 0; c0 < D / 8; c0 += 8) {
-                uint4 kv[8];
-#pragma unroll
-                for (int c = 0; c < 8; ++c) kv[c] = row >= 0 ? __ldg(kr + c0 + c) : make_uint4(0u, 0u, 0u, 0u);
-#pragma unroll
-                for (int c = 0; c < 8; ++c)
-#pragma unroll
-                    for (int hh = 0; hh < G; ++hh) {
-                        const uint4 w = __ldg(q + hh * (D / 8) + c0 + c);
-                        s[hh] = fma2_bf16(kv[c].w, w.w, fma2_bf16(kv[c].z, w.z, fma2_bf16(kv[c].y, w.y, fma2_bf16(kv[c].x, w.x, s[hh]))));
-                    }
-            }
-#pragma unroll
-            for (int hh = 0; hh < G; ++hh) {
-                s[hh] = row >= 0 ? __fmul_rn(s[hh], scale2) : NEG_INF;
-                if (A.own != nullptr) {
-                    const bool on = ((unsigned)own >> lane) & 1u;
-                    const float v = __shfl_sync(0xffffffffu, s[hh], __popc((unsigned)own & ((1u << lane) - 1u)));
-                    A.own[((size_t)t * A.Hq + g * G + hh) * 32 + lane] = on ? v : NEG_INF;
-                }
-                float mx = s[hh];
-#pragma unroll
-                for (int k = 16; k > 0; k >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, k));
-                mx = fmaxf(mx, m[hh]);
-                const float c = m[hh] == NEG_INF ? 0.f : ex2(m[hh] - mx);
-                const float p = s[hh] == NEG_INF ? 0.f : ex2(s[hh] - mx);
-                l[hh] = l[hh] * c + warp_sum(p);
-                m[hh] = mx;
-                s[hh] = p;
-#pragma unroll
-                for (int e = 0; e < E; ++e) o[hh][e] *= c;
-            }
+            for (int i = 0; i < 4; ++i) o[c][i][0] = o[c][i][1] = 0.f;
 #pragma unroll 1
-            for (int k0 = 0; k0 < 32; k0 += VB) {
-                if (k0 >= n - j0) break;
-                uint32_t v[VB][E / 2];
+        for (int j0 = 0; j0 < n; j0 += 32) {
+            int row[4], place[4];
 #pragma unroll
-                for (int k = 0; k < VB; ++k) {  // (a key outside has weight 0 over zeros)
-                    const int r = __shfl_sync(0xffffffffu, row, k0 + k);
-                    const bf16* vr = Vg + (size_t)max(r, 0) * A.rs + lane * E;
-                    if (E == 4) {
-                        const uint2 x = r >= 0 ? __ldg(reinterpret_cast<const uint2*>(vr)) : make_uint2(0u, 0u);
-                        v[k][0] = x.x, v[k][E / 2 - 1] = x.y;
+            for (int k = 0; k < 4; ++k) {
+                const int j = j0 + y + 8 * k;
+                row[k] = -1, place[k] = 0;
+                if (j < n) {
+                    if (A.rw != nullptr) {
+                        row[k] = own + (i0 + j) * P.W;
                     } else {
-                        v[k][0] = r >= 0 ? __ldg(reinterpret_cast<const uint32_t*>(vr)) : 0u;
-                    }
-                }
-#pragma unroll
-                for (int k = 0; k < VB; ++k)
-#pragma unroll
-                    for (int hh = 0; hh < G; ++hh) {
-                        const float p = __shfl_sync(0xffffffffu, s[hh], k0 + k);
-#pragma unroll
-                        for (int e = 0; e < E; e += 2) {
-                            o[hh][e] = fmaf(p, bf_lo(v[k][e / 2]), o[hh][e]);
-                            o[hh][e + 1] = fmaf(p, bf_hi(v[k][e / 2]), o[hh][e + 1]);
+                        place[k] = bit_place((unsigned)own, j);
+                        row[k] = P.n0 + place[k];
+                        if (A.tbl != nullptr) row[k] = A.tbl[row[k]];
+                        if (row[k] < 0 || row[k] >= A.cap) {
+                            b2_fail(B2_ERR_DOMAIN);
+                            row[k] = -1;
                         }
                     }
+                }
+            }
+            uint4 kv[4][C], vv[2][C];
+            auto load = [&](const bf16* from, int k, int c) {
+                return row[k] >= 0 ? __ldg(reinterpret_cast<const uint4*>(from + (size_t)row[k] * A.rs + c * 32)) : make_uint4(0u, 0u, 0u, 0u);
+            };
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+#pragma unroll
+                for (int c = 0; c < C; ++c) kv[k][c] = load(Kg, k, c);
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+#pragma unroll
+                for (int c = 0; c < C; ++c) vv[k][c] = load(Vg, k, c);
+            float s[2][4];
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+                s[b][0] = s[b][1] = s[b][2] = s[b][3] = 0.f;
+#pragma unroll
+                for (int c = 0; c < C; ++c) {
+                    const uint4 k0 = kv[2 * b][c], k1 = kv[2 * b + 1][c];
+                    mma16816(s[b], k0.x, k1.x, k0.y, k1.y, q[c].x, q[c].y);
+                    mma16816(s[b], k0.z, k1.z, k0.w, k1.w, q[c].z, q[c].w);
+                }
+            }
+            float f[2], p[2][4];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {  // head 2 x + e: key y + 8 k's score in s[k / 2][2 (k % 2) + e]
+                float mx = m[e];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    float& v = s[k >> 1][2 * (k & 1) + e];
+                    v = row[k] >= 0 ? __fmul_rn(v, scale2) : NEG_INF;
+                    mx = fmaxf(mx, v);
+                    if (scores != nullptr && 2 * x + e < G && row[k] >= 0) scores[(2 * x + e) * 32 + place[k]] = v;
+                }
+#pragma unroll
+                for (int k = 4; k < 32; k <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, k));
+                const float sub = mx == NEG_INF ? 0.f : mx;
+                f[e] = m[e] == NEG_INF ? 0.f : ex2(m[e] - sub);
+                float sum = 0.f;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const float w = ex2(s[k >> 1][2 * (k & 1) + e] - sub);
+                    p[k >> 1][2 * (k & 1) + e] = w, sum += w;
+                }
+#pragma unroll
+                for (int k = 4; k < 32; k <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, k);
+                l[e] = l[e] * f[e] + sum;
+                m[e] = mx;
+            }
+            const float f0 = __shfl_sync(0xffffffffu, f[0], y >> 1), f1 = __shfl_sync(0xffffffffu, f[1], y >> 1), fy = y & 1 ? f1 : f0;  // head y's
+#pragma unroll
+            for (int c = 0; c < C; ++c)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) o[c][i][0] *= fy, o[c][i][1] *= fy;
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+                uint32_t w0, w1;
+                asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w0) : "f"(p[b][1]), "f"(p[b][0]));
+                asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w1) : "f"(p[b][3]), "f"(p[b][2]));
+                const uint32_t a0 = turned(w0), a2 = turned(w1);
+#pragma unroll
+                for (int c = 0; c < C; ++c) {
+                    const uint32_t u0[4] = {vv[0][c].x, vv[0][c].y, vv[0][c].z, vv[0][c].w}, u1[4] = {vv[1][c].x, vv[1][c].y, vv[1][c].z, vv[1][c].w};
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        float d[4] = {o[c][i][0], o[c][i][1], 0.f, 0.f};
+                        mma16816(d, a0, 0u, a2, 0u, turned(u0[i]), turned(u1[i]));
+                        o[c][i][0] = d[0], o[c][i][1] = d[1];
+                    }
+                }
+                if (b == 0) {
+#pragma unroll
+                    for (int k = 0; k < 2; ++k)
+#pragma unroll
+                        for (int c = 0; c < C; ++c) vv[k][c] = load(Vg, k + 2, c);
+                }
             }
         }
         const size_t at = (size_t)(A.unit_row + u * G);
 #pragma unroll
-        for (int hh = 0; hh < G; ++hh) {
-            if (lane == 0) A.part_ml[at + hh] = make_float2(m[hh], l[hh]);
-            float* to = A.part_o + (at + hh) * D + lane * E;
-            if (E == 4) *reinterpret_cast<float4*>(to) = make_float4(o[hh][0], o[hh][1], o[hh][E - 2], o[hh][E - 1]);
-            else *reinterpret_cast<float2*>(to) = make_float2(o[hh][0], o[hh][E - 1]);
+        for (int e = 0; e < 2; ++e)
+            if (y == 0 && 2 * x + e < G) A.part_ml[at + 2 * x + e] = make_float2(m[e], l[e]);
+        if (y < G) {
+#pragma unroll
+            for (int c = 0; c < C; ++c) {
+                float4* to = reinterpret_cast<float4*>(A.part_o + (at + y) * D + c * 32 + x * 8);
+                to[0] = make_float4(o[c][0][0], o[c][0][1], o[c][1][0], o[c][1][1]);
+                to[1] = make_float4(o[c][2][0], o[c][2][1], o[c][3][0], o[c][3][1]);
+            }
         }
     }
 }
@@ -683,25 +730,35 @@ __global__ void __launch_bounds__(TW * 32, 1)
             if (p.tiles == 0) break;
             at = p.end;
             const int x = p.head * X.col_mul, y0 = p.head * X.row_mul;
+            // sixteen lanes four rows each (each half of the lanes 64 columns); past the tile's keys the last one again (its
+            // weight there is 0: the values multiplied by it must be ones that the rows see)
+            auto rows_of = [&](int i, int* r) {
+                const int keys = min(KT, p.keys - i * KT);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const int j = p.start + i * KT + min((lane & 15) * 4 + k, keys - 1);
+                    r[k] = A.tbl != nullptr ? A.tbl[j] : j;
+                }
+            };
+            int ahead[4];
+            rows_of(0, ahead);
 #pragma unroll 1
             for (int i = 0; i < p.tiles && ok; ++i) {
-                const int keys = min(KT, p.keys - i * KT);
-                const bool box = keys == KT && A.tbl == nullptr;
                 int y[4];
-                if (!box) {
-                    // sixteen lanes four rows each (and each half of them 64 columns); past the tile's keys the last one again
-                    // (its weight there is 0: the values multiplied by it must be ones that the rows see)
+                bool in_line = p.keys - i * KT >= KT;
+                const int r0 = __shfl_sync(0xffffffffu, ahead[0], 0);
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        const int j = p.start + i * KT + min((lane & 15) * 4 + k, keys - 1);
-                        int r = A.tbl != nullptr ? A.tbl[j] : j;
-                        if (r < 0 || r >= A.cap) {
-                            b2_fail(B2_ERR_DOMAIN);
-                            r = 0;
-                        }
-                        y[k] = y0 + r;
+                for (int k = 0; k < 4; ++k) {
+                    int r = ahead[k];
+                    in_line = in_line && r == r0 + (lane & 15) * 4 + k;
+                    if (r < 0 || r >= A.cap) {
+                        b2_fail(B2_ERR_DOMAIN);
+                        r = 0, in_line = false;
                     }
+                    y[k] = y0 + r;
                 }
+                const bool box = __all_sync(0xffffffffu, in_line);  // 64 rows one after the other: one copy
+                if (i + 1 < p.tiles) rows_of(i + 1, ahead);
 #pragma unroll
                 for (int kv = 0; kv < 2; ++kv) {
                     if (asked[kv] >= X.stages && !(ok = wait_or_fail(kv == 0 ? &sy.kempty[st] : &sy.vempty[st], ph, sy))) break;
@@ -709,7 +766,7 @@ __global__ void __launch_bounds__(TW * 32, 1)
                     if (lane == 0) mbar_expect_tx(bar, TILE);
                     __syncwarp();
                     if (box) {
-                        if (lane < D / 64) tma_box(dst + lane * HALF, kv == 0 ? &kbox : &vbox, x + lane * 64, y0 + p.start + i * KT, bar);
+                        if (lane < D / 64) tma_box(dst + lane * HALF, kv == 0 ? &kbox : &vbox, x + lane * 64, y0 + r0, bar);
                     } else if (lane < D / 4) {
                         tma_rows4(dst + (lane >> 4) * HALF + (lane & 15) * 512, kv == 0 ? &krows : &vrows, x + (lane >> 4) * 64, y, bar);
                     }
@@ -800,8 +857,8 @@ constexpr int KEEP_ROWS = 16;              // a kv head's queries (T G) up to wh
 struct States {
     long long p_row, u_row;
     int np, n, step, G;
-    __device__ __forceinline__ States(const LongArgs& A, int t, int g, int G_) : G(G_) {
-        const int4 a = __ldcg(A.info + 2 * t), b = __ldcg(A.info + 2 * t + 1);  // place, tiles, row, units; unit, line, rows, units
+    // a: place, tiles, row, units; b: unit, line, rows, units
+    __device__ __forceinline__ States(const LongArgs& A, const int4 a, const int4 b, int g, int G_) : G(G_) {
         const int place = g * b.y + a.x;
         int c = 0;
         np = 0, step = A.T * G;
@@ -851,68 +908,79 @@ __global__ void __launch_bounds__(JT) long_join(const LongArgs A, int weight_blo
     __shared__ float s_lse[KEEP_ROWS];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     pdl_launch_dependents();
-    pdl_wait();
     if ((int)blockIdx.x < A.T * A.Hk) {
         const int t = blockIdx.x / A.Hk, g = blockIdx.x - t * A.Hk, hh = warp / WH, sub = warp - hh * WH, head = g * G + hh;
-        const States S(A, t, g, G);
-        if (S.n == 0) return;  // padding, or refused
-        float M, L;
-        row_stats(A, S, head, hh, M, L, fac[warp]);
-        __syncwarp();
-        float o[E];
-#pragma unroll
-        for (int e = 0; e < E; ++e) o[e] = 0.f;
-        constexpr int B = 8;  // states in flight
+        float M, L, o[E];
+        // Twice: first, while the tiles are still at work, over places of the workspace whose contents are of no interest, so
+        // that the instructions are on the SM when the states are (2 us of a short pass's 10 were their first fetch).
 #pragma unroll 1
-        for (int k0 = sub; k0 < S.n; k0 += B * WH) {
-            float v[B][E];
+        for (int real = 0; real < 2; ++real) {
+            int4 a = make_int4(0, 1, 0, 1), b = make_int4(0, 1, 1, 1);
+            if (real) {
+                pdl_wait();
+                a = __ldcg(A.info + 2 * t), b = __ldcg(A.info + 2 * t + 1);
+            }
+            const States S(A, a, b, g, G);
+            if (S.n == 0) return;  // padding, or refused
+            row_stats(A, S, head, hh, M, L, fac[warp]);
+            __syncwarp();
 #pragma unroll
-            for (int j = 0; j < B; ++j) {
-                const int k = min(k0 + j * WH, S.n - 1);
-                const float* src = A.part_o + (size_t)(S.at(k) + hh) * D + lane * E;
-                if (E == 4) {
-                    const float4 x = __ldcg(reinterpret_cast<const float4*>(src));
-                    v[j][0] = x.x, v[j][1] = x.y, v[j][E - 2] = x.z, v[j][E - 1] = x.w;
-                } else {
-                    const float2 x = __ldcg(reinterpret_cast<const float2*>(src));
-                    v[j][0] = x.x, v[j][E - 1] = x.y;
+            for (int e = 0; e < E; ++e) o[e] = 0.f;
+            constexpr int B = 8;  // states in flight
+#pragma unroll 1
+            for (int k0 = sub; k0 < S.n; k0 += B * WH) {
+                float v[B][E];
+#pragma unroll
+                for (int j = 0; j < B; ++j) {
+                    const float* src = A.part_o + (size_t)(S.at(min(k0 + j * WH, S.n - 1)) + hh) * D + lane * E;
+                    if (E == 4) {
+                        const float4 x = __ldcg(reinterpret_cast<const float4*>(src));
+                        v[j][0] = x.x, v[j][1] = x.y, v[j][E - 2] = x.z, v[j][E - 1] = x.w;
+                    } else {
+                        const float2 x = __ldcg(reinterpret_cast<const float2*>(src));
+                        v[j][0] = x.x, v[j][E - 1] = x.y;
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < B; ++j) {
+                    if (k0 + j * WH >= S.n) break;
+                    const float f = fac[warp][k0 + j * WH];
+#pragma unroll
+                    for (int e = 0; e < E; ++e) o[e] = fmaf(f, v[j][e], o[e]);
                 }
             }
+            if (WH > 1) {
 #pragma unroll
-            for (int j = 0; j < B; ++j) {
-                if (k0 + j * WH >= S.n) break;
-                const float f = fac[warp][k0 + j * WH];
+                for (int e = 0; e < E; ++e) part[warp][lane * E + e] = o[e];
+                __syncthreads();
+                if (sub == 0)
+                    for (int w = 1; w < min(WH, S.n); ++w)
 #pragma unroll
-                for (int e = 0; e < E; ++e) o[e] = fmaf(f, v[j][e], o[e]);
+                        for (int e = 0; e < E; ++e) o[e] += part[warp + w][lane * E + e];
+                __syncthreads();
             }
         }
-        if (WH > 1) {
-#pragma unroll
-            for (int e = 0; e < E; ++e) part[warp][lane * E + e] = o[e];
-            __syncthreads();
-            if (sub != 0) return;
-            for (int w = 1; w < min(WH, S.n); ++w)
-#pragma unroll
-                for (int e = 0; e < E; ++e) o[e] += part[warp + w][lane * E + e];
-        }
+        if (sub != 0) return;
         if (lane == 0 && A.lse != nullptr) A.lse[(size_t)t * A.Hq + head] = M + log2f(L);
         bf16* out = A.out + ((size_t)t * A.Hq + head) * D + lane * E;
+        const float inv = __fdiv_rn(1.f, L);
 #pragma unroll
         for (int e = 0; e < E; e += 2) {
             __nv_bfloat162 v;
-            v.x = f2bf(__fdiv_rn(o[e], L)), v.y = f2bf(__fdiv_rn(o[e + 1], L));
+            v.x = f2bf(o[e] * inv), v.y = f2bf(o[e + 1] * inv);
             *reinterpret_cast<__nv_bfloat162*>(out + e) = v;
         }
         return;
     }
     // ---- the weights ------------------------------------------------------------------------------------------------------
+    pdl_wait();
     const int b = blockIdx.x - A.T * A.Hk, g = b / weight_blocks, n0 = __ldcg(A.n0p);
     const int n = n0 < 0 || n0 > A.cap - A.T ? -1 : n0 + (A.T == 1);  // keys whose scores were kept; -1: refused
     int j = (b - g * weight_blocks) * JT + threadIdx.x;
     if (n < 0 || (j - (int)threadIdx.x >= n && b != g * weight_blocks)) return;
     for (int r = warp; r < A.T * G; r += JW) {
         const int t = r / G, hh = r - t * G;
-        const States S(A, t, g, G);
+        const States S(A, __ldcg(A.info + 2 * t), __ldcg(A.info + 2 * t + 1), g, G);
         float M, L;
         row_stats(A, S, g * G + hh, hh, M, L, nullptr);
         if (lane == 0) s_lse[r] = M + log2f(L);
