@@ -922,14 +922,9 @@ __global__ void __launch_bounds__(JT) long_join(const LongArgs A, int weight_blo
             }
             const States S(A, a, b, g, G);
             if (S.n == 0) return;  // padding, or refused
-            row_stats(A, S, head, hh, M, L, fac[warp]);
-            __syncwarp();
-#pragma unroll
-            for (int e = 0; e < E; ++e) o[e] = 0.f;
-            constexpr int B = 8;  // states in flight
-#pragma unroll 1
-            for (int k0 = sub; k0 < S.n; k0 += B * WH) {
-                float v[B][E];
+            constexpr int B = 8;  // states in flight; the first ones are asked for before their factors are known
+            float v[B][E];
+            auto load = [&](int k0) {
 #pragma unroll
                 for (int j = 0; j < B; ++j) {
                     const float* src = A.part_o + (size_t)(S.at(min(k0 + j * WH, S.n - 1)) + hh) * D + lane * E;
@@ -941,12 +936,21 @@ __global__ void __launch_bounds__(JT) long_join(const LongArgs A, int weight_blo
                         v[j][0] = x.x, v[j][E - 1] = x.y;
                     }
                 }
+            };
+            load(sub);
+            row_stats(A, S, head, hh, M, L, fac[warp]);
+            __syncwarp();
 #pragma unroll
-                for (int j = 0; j < B; ++j) {
-                    if (k0 + j * WH >= S.n) break;
-                    const float f = fac[warp][k0 + j * WH];
+            for (int e = 0; e < E; ++e) o[e] = 0.f;
+#pragma unroll 1
+            for (int k0 = sub; k0 < S.n; k0 += B * WH) {
+                if (k0 != sub) load(k0);
 #pragma unroll
-                    for (int e = 0; e < E; ++e) o[e] = fmaf(f, v[j][e], o[e]);
+                for (int j = 0; j < B; ++j) {  // (no branch: the loads would sink below it, one after the other)
+                    const bool on = k0 + j * WH < S.n;
+                    const float f = on ? fac[warp][on ? k0 + j * WH : 0] : 0.f;
+#pragma unroll
+                    for (int e = 0; e < E; ++e) o[e] = fmaf(f, on ? v[j][e] : 0.f, o[e]);
                 }
             }
             if (WH > 1) {
