@@ -1019,7 +1019,7 @@ __global__ void __launch_bounds__(WT) long_weights(const __grid_constant__ CUten
     extern __shared__ __align__(1024) uint8_t smem[];
     __shared__ __align__(8) uint64_t full, done;
     __shared__ uint32_t tmem_slot;
-    __shared__ float s_lse[256];
+    __shared__ float s_lse[256], s_own[4][32];
     const int G = A.Hq / A.Hk, rows = A.T * G, N = (rows + 31) & ~31, g = blockIdx.y;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t sk = smem_u32(smem), sq = sk + TILE, cols = N > 128 ? 256u : N > 64 ? 128u : N > 32 ? 64u : 32u;
@@ -1096,11 +1096,17 @@ __global__ void __launch_bounds__(WT) long_weights(const __grid_constant__ CUten
             pdl_wait();
             for (int r = threadIdx.x; r < rows; r += WT) s_lse[r] = A.lse[(size_t)(r / G) * A.Hq + g * G + r % G];
             __syncthreads();
-            if (blockIdx.x == 0 && (int)threadIdx.x < A.T) {  // the pass's own rows: set
+            if (blockIdx.x == 0) {  // the pass's own rows: set; a lane a row, each warp a quarter of the queries
+                const int each = (rows + 3) / 4, lo = warp * each, hi = min(lo + each, rows);
                 float a = 0.f;
-#pragma unroll 8
-                for (int r = 0; r < rows; ++r) a += ex2(A.own[((size_t)(r / G) * A.Hq + g * G + r % G) * 32 + threadIdx.x] - s_lse[r]);
-                tot[n0 + threadIdx.x] = a;
+#pragma unroll 16
+                for (int r = lo; r < hi; ++r) {
+                    const int t = r / G;
+                    a += ex2(__ldcg(A.own + ((size_t)t * A.Hq + g * G + r - t * G) * 32 + lane) - s_lse[r]);
+                }
+                s_own[warp][lane] = a;
+                __syncthreads();
+                if ((int)threadIdx.x < A.T) tot[n0 + lane] = (s_own[0][lane] + s_own[1][lane]) + (s_own[2][lane] + s_own[3][lane]);
             }
             first = false;
         }
