@@ -851,6 +851,7 @@ __global__ void __launch_bounds__(TW * 32, 1)
 // ---- a row's parts joined ------------------------------------------------------------------------------------------------
 constexpr int JT = 256, JW = JT / 32;      // threads and warps of a block
 constexpr int STATES_MAX = CTAS_MAX + 64;  // a row's parts and units
+constexpr int WEIGHT_KEYS = 4 * JT;         // keys of a block that adds up weights
 constexpr int KEEP_ROWS = 16;              // a kv head's queries (T G) up to which a pass keeps its scores for the weights
 
 // where the states of (row t, kv head g) lie: state k of query head hh in row at(k) + hh
@@ -898,7 +899,7 @@ __device__ __forceinline__ void row_stats(const LongArgs& A, const States& S, in
 
 // The first T Hk blocks join one (row, kv head) each: JW / G warps a query head, each every so many-th state, a lane D / 32
 // dims, their sums added in order. The blocks after them, where a pass of few rows kept its scores, add up what it gives each
-// cache row: a thread a key, 2^(score - log2 of the row's denominator) over the kv head's queries in order - one sum in one
+// cache row: a thread four keys, 2^(score - log2 of the row's denominator) over the kv head's queries in order - one sum in one
 // order.
 template <int D, int G>
 __global__ void __launch_bounds__(JT) long_join(const LongArgs A, int weight_blocks) {
@@ -980,9 +981,19 @@ __global__ void __launch_bounds__(JT) long_join(const LongArgs A, int weight_blo
     pdl_wait();
     const int b = blockIdx.x - A.T * A.Hk, g = b / weight_blocks, n0 = __ldcg(A.n0p);
     const int n = n0 < 0 || n0 > A.cap - A.T ? -1 : n0 + (A.T == 1);  // keys whose scores were kept; -1: refused
-    int j = (b - g * weight_blocks) * JT + threadIdx.x;
-    if (n < 0 || (j - (int)threadIdx.x >= n && b != g * weight_blocks)) return;
-    for (int r = warp; r < A.T * G; r += JW) {
+    const int j0 = (b - g * weight_blocks) * WEIGHT_KEYS;
+    if (n < 0 || (j0 >= n && j0 > 0)) return;
+    const int rows = A.T * G;
+    const float* from = A.scores + (size_t)g * rows * A.score_n + threadIdx.x * 4;
+    float4 s[8];  // (the first scores asked for before the denominators are made)
+    auto load = [&](int j, int r0) {
+#pragma unroll
+        for (int r = 0; r < 8; ++r)
+            s[r] = r0 + r < rows && j + (int)threadIdx.x * 4 < n ? __ldcg(reinterpret_cast<const float4*>(from + (size_t)(r0 + r) * A.score_n + j))
+                                                                  : make_float4(NEG_INF, NEG_INF, NEG_INF, NEG_INF);
+    };
+    load(j0, 0);
+    for (int r = warp; r < rows; r += JW) {
         const int t = r / G, hh = r - t * G;
         const States S(A, __ldcg(A.info + 2 * t), __ldcg(A.info + 2 * t + 1), g, G);
         float M, L;
@@ -991,17 +1002,28 @@ __global__ void __launch_bounds__(JT) long_join(const LongArgs A, int weight_blo
     }
     __syncthreads();
     float* tot = A.totals + (size_t)g * A.ts;
-    if (A.T > 1 && b == g * weight_blocks && (int)threadIdx.x < A.T) {  // the pass's own rows: set
-        float a = 0.f;
-        for (int r = 0; r < A.T * G; ++r)
-            a += ex2(A.own[((size_t)(r / G) * A.Hq + g * G + r % G) * 32 + threadIdx.x] - s_lse[r]);
-        tot[n0 + threadIdx.x] = a;
-    }
-    for (; j < n; j += weight_blocks * JT) {
+    if (A.T > 1 && j0 == 0 && (int)threadIdx.x < A.T) {  // the pass's own rows: set
         float a = 0.f;
 #pragma unroll 8
-        for (int r = 0; r < A.T * G; ++r) a += ex2(A.scores[((size_t)g * A.T * G + r) * A.score_n + j] - s_lse[r]);
-        tot[j] = j < n0 ? tot[j] + a : a;
+        for (int r = 0; r < rows; ++r) a += ex2(__ldcg(A.own + ((size_t)(r / G) * A.Hq + g * G + r % G) * 32 + threadIdx.x) - s_lse[r]);
+        tot[n0 + threadIdx.x] = a;
+    }
+    for (int j = j0; j < n; j += weight_blocks * WEIGHT_KEYS) {
+        float a[4] = {0.f, 0.f, 0.f, 0.f};
+        for (int r0 = 0; r0 < rows; r0 += 8) {
+            if (j != j0 || r0 != 0) load(j, r0);
+#pragma unroll
+            for (int r = 0; r < 8; ++r) {
+                if (r0 + r >= rows) break;
+                const float d = s_lse[r0 + r];
+                a[0] += ex2(s[r].x - d), a[1] += ex2(s[r].y - d), a[2] += ex2(s[r].z - d), a[3] += ex2(s[r].w - d);
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int at = j + threadIdx.x * 4 + k;
+            if (at < n) tot[at] = at < n0 ? tot[at] + a[k] : a[k];
+        }
     }
 }
 
@@ -1218,8 +1240,8 @@ int launch_long(const LongArgs& a, cudaStream_t s) {
     if (const int rc = b2_allow_smem(reinterpret_cast<const void*>(tiles), tiles_allowed)) return rc;
     if (const int rc = launch(tiles, dim3(a.ctas), dim3(TW * 32), (size_t)queries + (size_t)2 * x.stages * tile, s, tm[0], tm[1], tm[2], tm[3], x))
         return rc;
-    // (blocks enough for a key a thread of the whole cache, or for the card)
-    const int wb = a.scores != nullptr ? min((a.cap + JT - 1) / JT, max(1, 8 * a.ctas / a.Hk)) : 0;
+    // (blocks enough for the whole cache, or for the card)
+    const int wb = a.scores != nullptr ? min((a.cap + WEIGHT_KEYS - 1) / WEIGHT_KEYS, max(1, 4 * a.ctas / a.Hk)) : 0;
     if (const int rc = launch(long_join<D, G>, dim3(a.T * a.Hk + wb * a.Hk), dim3(JT), 0, s, a, wb)) return rc;
     if (a.totals == nullptr || a.scores != nullptr) return B2_OK;
     auto weights = long_weights<D>;
