@@ -194,25 +194,26 @@ __device__ __noinline__ Part part_at(const Plan& P, int span, int at, int stop, 
 // part's end) or on the two halves of an item's up to 256 rows. Tensor memory, 512 columns: two score tiles of 64 columns a
 // warpgroup, so that the next one is there when a warpgroup comes from the last, then the two outputs; weights (bf16) lie over
 // their scores.
-__device__ __forceinline__ uint64_t desc_sw128(uint32_t saddr, uint32_t lbo) {
-    return (uint64_t)((saddr & 0x3FFFFu) >> 4) | ((uint64_t)(lbo >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) |
-           ((uint64_t)2 << 61);
-}
+// the low word of a shared-memory operand's descriptor: where it begins and, for the values, the step to their next 64 dims
+__device__ __forceinline__ uint32_t desc_sw128(uint32_t saddr, uint32_t lbo) { return ((saddr & 0x3FFFFu) >> 4) | ((lbo >> 4) << 16); }
+// (a descriptor's upper word is the same for every operand here: 1024 bytes between 8-row groups, version 1, 128-byte swizzle)
+constexpr uint32_t DESC_HI = (1024u >> 4) | (1u << 14) | (2u << 29);
 // The MMAs are issued by one elected lane (`lead` nonzero in it) of a warp whose lanes all walk the same code: the operands
-// then are warp-uniform values, which the instruction wants, and not one lane's.
+// then are warp-uniform values, which the instruction wants (by one lane in a branch of its own the longest pass took 67 us
+// against 58).
 __device__ __forceinline__ uint32_t elect_lane() {
     uint32_t on;
     asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.u32 %0, 1, 0, p;\n}\n" : "=r"(on));
     return on;
 }
-__device__ __forceinline__ void mma_ss(uint32_t lead, uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
-    asm volatile("{\n.reg .pred p, q;\nsetp.ne.b32 p, %4, 0;\nsetp.ne.b32 q, %5, 0;\n"
-                 "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc), "r"(lead)
+__device__ __forceinline__ void mma_ss(uint32_t lead, uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile("{\n.reg .pred p, q;\n.reg .b64 da, db;\nsetp.ne.b32 p, %4, 0;\nsetp.ne.b32 q, %5, 0;\nmov.b64 da, {%1, %6};\nmov.b64 db, {%2, %6};\n"
+                 "@q tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n}\n" ::"r"(d), "r"(a), "r"(b), "r"(idesc), "r"(acc), "r"(lead), "n"(DESC_HI)
                  : "memory");
 }
-__device__ __forceinline__ void mma_ts(uint32_t lead, uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
-    asm volatile("{\n.reg .pred p, q;\nsetp.ne.b32 p, %4, 0;\nsetp.ne.b32 q, %5, 0;\n"
-                 "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(acc), "r"(lead)
+__device__ __forceinline__ void mma_ts(uint32_t lead, uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile("{\n.reg .pred p, q;\n.reg .b64 db;\nsetp.ne.b32 p, %4, 0;\nsetp.ne.b32 q, %5, 0;\nmov.b64 db, {%2, %6};\n"
+                 "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, p;\n}\n" ::"r"(d), "r"(a), "r"(b), "r"(idesc), "r"(acc), "r"(lead), "n"(DESC_HI)
                  : "memory");
 }
 __device__ __forceinline__ void mma_commit(uint32_t lead, uint32_t bar) {
@@ -220,6 +221,8 @@ __device__ __forceinline__ void mma_commit(uint32_t lead, uint32_t bar) {
                  "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}\n" ::"r"(bar), "r"(lead)
                  : "memory");
 }
+__device__ __forceinline__ void tm_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tm_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 // two f32 side by side: one instruction for both
 __device__ __forceinline__ uint64_t pair2(float x, float y) {
     uint64_t v;
@@ -237,8 +240,6 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b));
     return v;
 }
-__device__ __forceinline__ void tm_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void tm_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tm_ld32(uint32_t addr, uint32_t* r) {
     asm volatile(
         "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
@@ -500,6 +501,65 @@ __device__ __forceinline__ void own_units(const LongArgs& A, const Plan& P, int 
     }
 }
 
+// where the issuing warp stands: the stages' descriptors and numbers, and the phases - of either ring, and of the weights'
+// and the products' buffers, a bit each (2 w + b)
+struct Issuer {
+    uint32_t k, v;
+    int ks, vs;
+    uint32_t kph, vph, pph;
+};
+
+// The MMAs of one part: job j is tile j for warpgroup j & 1 (NRT 1), or its half of tile j / 2's query rows (NRT 2);
+// scores run four jobs ahead of the products with the values, over the weights of the warpgroup's last tile but one.
+// D f32, A and B bf16; S: both K-major, N = 64 keys; O: the values' dims are B's N and lie contiguous, N = D.
+template <int D, int NRT>
+__device__ __forceinline__ bool issue_part(Issuer& is, TileSync& sy, uint32_t lead, uint32_t tmem, uint32_t q0, uint32_t k0, uint32_t v0, int stages, int jobs) {
+    constexpr int TILE = KT * D * 2, HALF = KT * 128, QTILE = 128 * D * 2, QHALF = 128 * 128;
+    constexpr uint32_t base_desc = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(128 >> 4) << 24);
+    constexpr uint32_t desc_s = base_desc | ((uint32_t)(KT >> 3) << 17), desc_o = base_desc | (1u << 16) | ((uint32_t)(D >> 3) << 17);
+    uint32_t k = is.k, v = is.v, kph = is.kph, vph = is.vph, pph = is.pph;
+    int ks = is.ks, vs = is.vs;
+#pragma unroll 1
+    for (int j0 = -4; j0 < jobs; j0 += 4) {
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const int w = u & 1, b = u >> 1, j = j0 + u;
+            constexpr bool one = NRT == 1;
+            if (j0 >= 0 && j < jobs) {  // job j's share of the output
+                if ((one || w == 0) && !wait_or_fail(&sy.vfull[vs], vph, sy)) return false;
+                if (!wait_or_fail(&sy.pready[w][b], (pph >> u) & 1, sy)) return false;
+                pph ^= 1u << u;
+                tm_after();
+#pragma unroll
+                for (int i = 0; i < KT / 16; ++i)
+                    mma_ts(lead, tmem + 256 + w * 128, tmem + w * 128 + b * KT + i * 8, v + i * (2048 >> 4), desc_o, i > 0 || j >= 2);
+                mma_commit(lead, smem_u32(&sy.pv[w][b]));
+                if (one || w == 1) {
+                    mma_commit(lead, smem_u32(&sy.vempty[vs]));
+                    v += TILE >> 4;
+                    if (++vs == stages) vs = 0, vph ^= 1, v = v0;
+                }
+            }
+            if (j + 4 < jobs) {  // the scores of job j + 4
+                if ((one || w == 0) && !wait_or_fail(&sy.kfull[ks], kph, sy)) return false;
+                tm_after();
+#pragma unroll
+                for (int i = 0; i < D / 16; ++i)
+                    mma_ss(lead, tmem + w * 128 + b * KT, q0 + (uint32_t)(((one ? 0 : w * QTILE) + (i >> 2) * QHALF + (i & 3) * 32) >> 4),
+                           k + (uint32_t)(((i >> 2) * HALF + (i & 3) * 32) >> 4), desc_s, i > 0);
+                mma_commit(lead, smem_u32(&sy.sfull[w][b]));
+                if (one || w == 1) {
+                    mma_commit(lead, smem_u32(&sy.kempty[ks]));
+                    k += TILE >> 4;
+                    if (++ks == stages) ks = 0, kph ^= 1, k = k0;
+                }
+            }
+        }
+    }
+    is.k = k, is.v = v, is.kph = kph, is.vph = vph, is.pph = pph, is.ks = ks, is.vs = vs;
+    return true;
+}
+
 template <int D, int G>
 __global__ void __launch_bounds__(TW * 32, 1)
     long_tiles(const __grid_constant__ CUtensorMap kbox, const __grid_constant__ CUtensorMap krows,
@@ -551,7 +611,7 @@ __global__ void __launch_bounds__(TW * 32, 1)
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
         const uint32_t ts = tmem + lanes + wg * 128, to = tmem + lanes + 256 + wg * 128;
         const float scale2 = fabsf(__fmul_rn(A.scale, LOG2E));  // (a negative scale's sign is the queries')
-        uint32_t count = 0;                                     // this warpgroup's tiles so far
+        uint32_t turn = 0;  // bit b: score buffer b's phase
         uint32_t stph = 0, nph = 0;
         bool ok = true;
         for (int at = begin; at < stop && ok;) {
@@ -592,9 +652,10 @@ __global__ void __launch_bounds__(TW * 32, 1)
                 keep = A.scores + ((size_t)p.head * p.rows + row) * A.score_n + p.start + wg * KT;
             float m = NEG_INF, l = 0.f;
 #pragma unroll 1
-            for (int i = 0; i < mine; ++i, ++count) {
-                const int b = count & 1;
-                if (!(ok = wait_or_fail(&sy.sfull[wg][b], (count >> 1) & 1, sy))) break;
+            for (int i = 0; i < mine; ++i) {
+                const int b = i & 1;
+                if (!(ok = wait_or_fail(&sy.sfull[wg][b], (turn >> b) & 1, sy))) break;
+                turn ^= 1u << b;
                 tm_after();
                 if (!idle) {
                     const int left = p.keys - (two ? i : 2 * i + wg) * KT;  // keys from this tile's first on
@@ -616,7 +677,7 @@ __global__ void __launch_bounds__(TW * 32, 1)
                     const float ref = i == 0 ? top : (top > m + 8.f ? top : m);
                     if (i > 0 && __any_sync(0xffffffffu, ref != m)) {
                         // (the product before must be in: the one before that is, these scores were asked for after it)
-                        if (!(ok = wait_or_fail(&sy.pv[wg][b ^ 1], ((count - 1) >> 1) & 1, sy))) break;
+                        if (!(ok = wait_or_fail(&sy.pv[wg][b ^ 1], ~(turn >> (b ^ 1)) & 1, sy))) break;
                         tm_after();
                         const float f = m == NEG_INF ? 0.f : ex2(m - ref);
                         l *= f;
@@ -665,7 +726,7 @@ __global__ void __launch_bounds__(TW * 32, 1)
                 if (lane == 0) mbar_arrive(smem_u32(&sy.pready[wg][b]));
             }
             // ---- the part's state ----------------------------------------------------------------------------------------
-            if (ok && mine > 0) ok = wait_or_fail(&sy.pv[wg][(count - 1) & 1], ((count - 1) >> 1) & 1, sy);
+            if (ok && mine > 0) ok = wait_or_fail(&sy.pv[wg][(mine - 1) & 1], ~(turn >> ((mine - 1) & 1)) & 1, sy);
             tm_after();
             if (!two && wg == 1) {
                 s_m[row] = m, s_l[row] = l;
@@ -786,57 +847,21 @@ __global__ void __launch_bounds__(TW * 32, 1)
         own_units<D, G>(A, plan, (warp - 10) * gridDim.x + blockIdx.x, OWN_WARPS * gridDim.x);
     } else {
         // ---- the MMAs -----------------------------------------------------------------------------------------------------------
-        // D f32, A and B bf16; S: both K-major, N = 64 keys; O: the values' dims are B's N and lie contiguous, N = D
-        constexpr uint32_t base_desc = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(128 >> 4) << 24);
-        constexpr uint32_t desc_s = base_desc | ((uint32_t)(KT >> 3) << 17), desc_o = base_desc | (1u << 16) | ((uint32_t)(D >> 3) << 17);
-        const uint64_t q0 = desc_sw128(sq, 0), k0 = desc_sw128(sk, 0), v0 = desc_sw128(sv, HALF);
-        const uint32_t lead = elect_lane();
-        int ks = 0, vs = 0;
-        uint32_t kph = 0, vph = 0, qph = 0, scount0 = 0, scount1 = 0, pcount0 = 0, pcount1 = 0;
+        // What a job costs this warp is its instructions, one after the other beside the weights' warps, so a buffer's and a
+        // warpgroup's numbers are constants of an unrolled turn of four jobs and addresses advance by additions.
+        const uint32_t lead = elect_lane(), q0 = desc_sw128(sq, 0), k0 = desc_sw128(sk, 0), v0 = desc_sw128(sv, HALF);
+        Issuer is{k0, v0, 0, 0, 0u, 0u, 0u};
+        uint32_t qph = 0;
         bool ok = true;
         for (int at = begin; at < stop && ok;) {
             const Part p = part_at<G>(plan, A.T * G, at, stop, blockIdx.x);
-            if (__shfl_sync(0xffffffffu, p.tiles, 0) == 0) break;
+            const int tiles = __shfl_sync(0xffffffffu, p.tiles, 0), rows = __shfl_sync(0xffffffffu, p.rows, 0);
+            if (tiles == 0) break;
             at = __shfl_sync(0xffffffffu, p.end, 0);
-            // job j: tile j for warpgroup j & 1, or both warpgroups' halves of tile j / 2; scores run four jobs ahead
-            const int nrt = __shfl_sync(0xffffffffu, p.rows, 0) > 128 ? 2 : 1, jobs = __shfl_sync(0xffffffffu, p.tiles, 0) * nrt;
             if (!(ok = wait_or_fail(&sy.qfull, qph, sy))) break;
             qph ^= 1;
-#pragma unroll 1
-            for (int j = -4; j < jobs; ++j) {
-                const int w = j & 1;  // (job j + 4's warpgroup too)
-                const bool begins = nrt == 1 || w == 0, ends = nrt == 1 || w == 1;  // its tile's first, last job
-                if (j >= 0) {  // job j's share of the output
-                    const uint32_t c = w ? pcount1++ : pcount0++, b = c & 1;
-                    if (begins && !(ok = wait_or_fail(&sy.vfull[vs], vph, sy))) break;
-                    if (!(ok = wait_or_fail(&sy.pready[w][b], (c >> 1) & 1, sy))) break;
-                    tm_after();
-                    const uint64_t bv = v0 + (uint64_t)(vs * (TILE >> 4));
-#pragma unroll
-                    for (int k = 0; k < KT / 16; ++k)
-                        mma_ts(lead, tmem + 256 + w * 128, tmem + w * 128 + b * KT + k * 8, bv + k * (2048 >> 4), desc_o, j >= 2 || k > 0);
-                    mma_commit(lead, smem_u32(&sy.pv[w][b]));
-                    if (ends) {
-                        mma_commit(lead, smem_u32(&sy.vempty[vs]));
-                        if (++vs == X.stages) vs = 0, vph ^= 1;
-                    }
-                }
-                if (j + 4 < jobs) {  // the scores of job j + 4, over the weights of the warpgroup's last but one
-                    const uint32_t b = (w ? scount1++ : scount0++) & 1;
-                    if (begins && !(ok = wait_or_fail(&sy.kfull[ks], kph, sy))) break;
-                    tm_after();
-                    const uint64_t qa = q0 + (uint64_t)(nrt == 2 ? w * (QTILE >> 4) : 0), kb = k0 + (uint64_t)(ks * (TILE >> 4));
-#pragma unroll
-                    for (int k = 0; k < D / 16; ++k)
-                        mma_ss(lead, tmem + w * 128 + b * KT, qa + (uint64_t)(((k >> 2) * QHALF + (k & 3) * 32) >> 4),
-                               kb + (uint64_t)(((k >> 2) * HALF + (k & 3) * 32) >> 4), desc_s, k > 0);
-                    mma_commit(lead, smem_u32(&sy.sfull[w][b]));
-                    if (ends) {
-                        mma_commit(lead, smem_u32(&sy.kempty[ks]));
-                        if (++ks == X.stages) ks = 0, kph ^= 1;
-                    }
-                }
-            }
+            ok = rows > 128 ? issue_part<D, 2>(is, sy, lead, tmem, q0, k0, v0, X.stages, 2 * tiles)
+                            : issue_part<D, 1>(is, sy, lead, tmem, q0, k0, v0, X.stages, tiles);
         }
         mma_commit(lead, smem_u32(&sy.drain));
         (void)mbar_wait_bounded(smem_u32(&sy.drain), 0);
@@ -1103,14 +1128,14 @@ __global__ void __launch_bounds__(WT) long_weights(const __grid_constant__ CUten
             ok = mbar_wait_bounded(smem_u32(&full), ph);
             ok = __all_sync(0xffffffffu, ok);
             if (ok) {
-                const uint32_t lead = elect_lane();
                 const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(WT >> 4) << 24);
-                const uint64_t ka = desc_sw128(sk, 0), qb = desc_sw128(sq, 0);
+                const uint32_t ka = desc_sw128(sk, 0), qb = desc_sw128(sq, 0);
                 tm_after();
+                const uint32_t lead = elect_lane();
 #pragma unroll
                 for (int k = 0; k < D / 16; ++k)
-                    mma_ss(lead, tmem, ka + (uint64_t)(((k >> 2) * HALF + (k & 3) * 32) >> 4),
-                           qb + (uint64_t)(((k >> 2) * (N * 128) + (k & 3) * 32) >> 4), idesc, k > 0);
+                    mma_ss(lead, tmem, ka + (uint32_t)(((k >> 2) * HALF + (k & 3) * 32) >> 4),
+                           qb + (uint32_t)(((k >> 2) * (N * 128) + (k & 3) * 32) >> 4), idesc, k > 0);
                 mma_commit(lead, smem_u32(&done));
             }
         }
