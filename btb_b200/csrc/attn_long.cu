@@ -35,6 +35,7 @@ struct LongArgs {
     long long score_n;
     float scale;
     int T, Hq, Hk, win, cap, ctas;
+    int own_share;  // warps that take a kv head's units, about
     long long hs, rs, ts;
 };
 
@@ -75,7 +76,7 @@ __device__ __forceinline__ int warp_excl(int v, int lane, int& total) {
 // units of a (row, kv head) at most: enough for every warp where rows and heads are few
 __host__ __device__ __forceinline__ int units_max(int T, int Hk) { return max(16, min(64, 1024 / (T * Hk))); }
 
-// one warp fills `P`; `tell`: this block records a refused layout and the rows' places for the joining kernel
+// one warp fills `P`; `tell`: this block records a refused layout
 template <int G>
 __device__ __forceinline__ void make_plan(const LongArgs& A, Plan& P, bool tell) {
     const int t = threadIdx.x & 31;
@@ -128,23 +129,28 @@ __device__ __forceinline__ void make_plan(const LongArgs& A, Plan& P, bool tell)
     const int p_at = warp_excl(p_tiles ? p_tiles + GAP : 0, t, line), p_row0 = warp_excl(p_tiles ? __popc(mask) * G : 0, t, pr);
     // units of about a warp's fair share of the own keys, a multiple of 32, no row in more of them than its room allows
     const int keys = __reduce_add_sync(0xffffffffu, min(own_n, 1 << 20));
-    int chunk = (int)(((long long)keys * A.Hk + A.ctas * OWN_WARPS - 1) / (A.ctas * OWN_WARPS));
     const int most = __reduce_max_sync(0xffffffffu, own_n), room = units_max(A.T, A.Hk);
-    chunk = (max(chunk, (most + room - 1) / room) + 31) & ~31;
+    const int chunk = (max((keys + A.own_share - 1) / A.own_share, (most + room - 1) / room) + 31) & ~31;
     const int unit0 = warp_excl(own_n > 0 ? (own_n + chunk - 1) / chunk : 0, t, units);
     P.mask[t] = mask, P.p_start[t] = start, P.p_count[t] = count, P.p_tiles[t] = p_tiles, P.p_at[t] = p_at, P.p_row0[t] = p_row0;
     P.lead[t] = lead, P.own[t] = own, P.own_n[t] = own_n, P.unit0[t] = unit0;
     const int src = lead < 0 ? 0 : lead;
     const int its = __shfl_sync(0xffffffffu, mask, src), before = __shfl_sync(0xffffffffu, p_row0, src);
-    const int some = __shfl_sync(0xffffffffu, p_tiles, src), at = __shfl_sync(0xffffffffu, p_at, src);
+    const int some = __shfl_sync(0xffffffffu, p_tiles, src);
     const int below = __popc(its & ((1u << t) - 1u));  // the row's place among its prefix's
     if (lead >= 0 && some > 0) P.order[before / G + below] = t;
-    if (tell && t < A.T) {  // for the joining kernel: where the row's states lie (none: padding, or refused)
-        A.info[2 * t] = make_int4(at, lead < 0 ? 0 : some, before + below * G, own_n > 0 ? (own_n + chunk - 1) / chunk : 0);
-        A.info[2 * t + 1] = make_int4(unit0, line, pr, units);
-    }
     if (t == 0) P.W = W, P.line = line, P.rows = pr, P.units = units, P.chunk = chunk, P.n0 = n0;
     __syncwarp();
+}
+// one warp writes for the joining kernel where each row's states lie (none: padding, or refused)
+template <int G>
+__device__ __forceinline__ void tell_plan(const LongArgs& A, const Plan& P) {
+    const int t = threadIdx.x & 31, lead = P.lead[t], l = max(lead, 0);
+    if (t >= A.T) return;
+    const int below = __popc(P.mask[l] & ((1u << t) - 1u));  // the row's place among its prefix's
+    const int units = P.own_n[t] > 0 ? (P.own_n[t] + P.chunk - 1) / P.chunk : 0;
+    A.info[2 * t] = make_int4(P.p_at[l], lead < 0 ? 0 : P.p_tiles[l], P.p_row0[l] + below * G, units);
+    A.info[2 * t + 1] = make_int4(P.unit0[t], P.line, P.rows, P.units);
 }
 
 // the even cut of the heads' line over the CTAs; no more of them than it is long, so that no stretch between two others is
@@ -621,23 +627,29 @@ __global__ void __launch_bounds__(TW * 32, 1)
             const bool two = p.rows > 128;
             {   // the part's queries into shared memory as the MMA reads them: 16-byte piece c of row r at c ^ (r & 7)
                 const uint32_t flip = A.scale < 0.f ? 0x80008000u : 0u;
-                uint4 v[2][D / 16];
+                // eight lanes a row's 128 bytes, four rows a warp at a time (a row a lane took 5500 cycles for 256 rows: every
+                // lane's piece another line)
+                const int x = lane & 7, n = two ? 8 : 4;  // the warp's runs of four rows of each of the D / 64 column blocks
+#pragma unroll 1
+                for (int i0 = 0; i0 < n; i0 += 4) {
+                    uint4 v[4][D / 64];
 #pragma unroll
-                for (int rt = 0; rt < 2; ++rt) {
-                    const int r = rt * 128 + row;
-                    const int t = r < p.rows ? plan.order[p.order + r / G] : 0;
-                    const uint4* src = reinterpret_cast<const uint4*>(A.q + ((size_t)t * A.Hq + p.head * G + r % G) * D) + wg * (D / 16);
+                    for (int i = 0; i < 4; ++i) {
+                        const int r = (i0 + i) * 32 + warp * 4 + (lane >> 3);
+                        const int t = r < p.rows ? plan.order[p.order + r / G] : 0;
+                        const uint4* src = reinterpret_cast<const uint4*>(A.q + ((size_t)t * A.Hq + p.head * G + r % G) * D) + x;
 #pragma unroll
-                    for (int c = 0; c < D / 16; ++c) v[rt][c] = r < p.rows ? src[c] : make_uint4(0u, 0u, 0u, 0u);
-                }
+                        for (int c = 0; c < D / 64; ++c) v[i][c] = r < p.rows ? src[c * 8] : make_uint4(0u, 0u, 0u, 0u);
+                    }
 #pragma unroll
-                for (int rt = 0; rt < 2; ++rt) {
-                    if (rt == 1 && !two) break;
+                    for (int i = 0; i < 4; ++i) {
+                        const int r = (i0 + i) * 32 + warp * 4 + (lane >> 3), rr = r & 127;
 #pragma unroll
-                    for (int c = 0; c < D / 16; ++c) {
-                        v[rt][c].x ^= flip, v[rt][c].y ^= flip, v[rt][c].z ^= flip, v[rt][c].w ^= flip;
-                        const int piece = wg * (D / 16) + c;
-                        *reinterpret_cast<uint4*>(smem + rt * QTILE + (piece >> 3) * QHALF + row * 128 + (((piece & 7) ^ (row & 7)) << 4)) = v[rt][c];
+                        for (int c = 0; c < D / 64; ++c) {
+                            uint4 w = v[i][c];
+                            w.x ^= flip, w.y ^= flip, w.z ^= flip, w.w ^= flip;
+                            *reinterpret_cast<uint4*>(smem + (r >> 7) * QTILE + c * QHALF + rr * 128 + ((x ^ (rr & 7)) << 4)) = w;
+                        }
                     }
                 }
                 fence_proxy_async();
@@ -844,6 +856,7 @@ __global__ void __launch_bounds__(TW * 32, 1)
                 if (uses > 0) (void)mbar_wait_bounded(smem_u32(kv == 0 ? &sy.kfull[s] : &sy.vfull[s]), (uint32_t)(uses - 1) & 1);
             }
     } else if (warp >= 10) {
+        if (warp == 10 && blockIdx.x == 0) tell_plan<G>(A, plan);
         own_units<D, G>(A, plan, (warp - 10) * gridDim.x + blockIdx.x, OWN_WARPS * gridDim.x);
     } else {
         // ---- the MMAs -----------------------------------------------------------------------------------------------------------
@@ -1327,6 +1340,7 @@ extern "C" int btb_b200_attn_shared(const void* q, const void* K, const void* V,
     a.q = static_cast<const bf16*>(q), a.K = static_cast<const bf16*>(K), a.V = static_cast<const bf16*>(V);
     a.out = static_cast<bf16*>(out), a.rw = static_cast<const int*>(rw), a.sinks = static_cast<const float*>(sinks);
     a.scale = scale, a.T = T, a.Hq = Hq, a.Hk = Hk, a.win = win, a.cap = cap, a.ctas = long_ctas(), a.hs = hs, a.rs = rs;
+    a.own_share = max(1, a.ctas * OWN_WARPS / Hk);
     (void)take_states(a, workspace, D);
     return D == 64 ? launch_long_g<64>(a, static_cast<cudaStream_t>(stream)) : launch_long_g<128>(a, static_cast<cudaStream_t>(stream));
 }
@@ -1350,6 +1364,7 @@ extern "C" int btb_b200_attn_scored(const void* q, const void* K, const void* V,
     a.tbl = static_cast<const int*>(tbl), a.sinks = static_cast<const float*>(sinks);
     a.totals = static_cast<float*>(totals), a.ts = ts;
     a.scale = scale, a.T = T, a.Hq = Hq, a.Hk = Hk, a.cap = cap, a.ctas = long_ctas(), a.hs = hs, a.rs = rs;
+    a.own_share = max(1, a.ctas * OWN_WARPS / Hk);
     a.lse = take_states(a, workspace, D), a.own = a.lse + (size_t)T * Hq;
     if (keeps_scores(T, Hq, Hk)) {
         const uintptr_t past = reinterpret_cast<uintptr_t>(a.own + (size_t)T * Hq * 32);
