@@ -48,7 +48,7 @@ struct LongArgs {
 // A row's own keys (its steps in the rows layout, its path in a chain or tree pass) are no one else's: units of up to
 // `chunk` keys of one (row, kv head), a warp each, beside the tiles. A one-row pass's own key joins its prefix.
 constexpr int KT = 64;         // keys a tile
-constexpr int GAP = 4;
+constexpr int GAP = 8;  // (4: 52.6 us where 8 takes 49.1, for 32 rows over 32768; shorter ones within 3 %)
 constexpr int CTAS_MAX = 160;  // CTAs of the tile kernel at most
 constexpr int OWN_WARPS = 2;   // warps of a CTA that take units (two more would leave all of them 128 registers)
 
@@ -1272,7 +1272,9 @@ int launch_long(const LongArgs& a, cudaStream_t s) {
     for (int k = 0; k < 4; ++k)
         if (const int rc = make_map(&tm[k], k < 2 ? a.K : a.V, rows, cols, a.rs, k & 1 ? 1 : KT)) return rc;
     const int tile = KT * D * 2, queries = (a.T * G > 128 ? 2 : 1) * 128 * D * 2;
-    x.stages = min((224 * 1024 - queries) / (2 * tile), STAGES_MAX);
+    // (16 KB short of what a block may have: the joining kernel's blocks then find room a little earlier. 8 rows over 2048 take
+    // 15.6 us so, else 16.5, 32 over 32768 47.4 and 49.1; one row over 32768, with a stage fewer, 38.1 and 37.5)
+    x.stages = min((208 * 1024 - queries) / (2 * tile), STAGES_MAX);
     auto tiles = long_tiles<D, G>;
     static bool tiles_allowed[64], weights_allowed[64];
     if (const int rc = b2_allow_smem(reinterpret_cast<const void*>(tiles), tiles_allowed)) return rc;

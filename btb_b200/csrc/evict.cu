@@ -28,7 +28,7 @@ struct EvictArgs {
     int* n_seen;          // n0 as the selection read it (n_out may be n0p's word)
     long long ls, ld, hs, rs;
     int layers, Hk, D, cap, cap_d, keep, recent;
-    int held;             // the totals of a head fit a block's shared memory
+    int held;             // the ranks of a head fit a block's shared memory
     int parts;            // evict_move: blocks that share a (layer, kv head, K or V): pieces of a row in place, else ranges of rows
     int in_place;
 };
@@ -47,7 +47,7 @@ constexpr int COPIES = 4;               // of the histogram: many rows have equa
 
 // The rank of the last kept total, eleven bits at a time from histograms of the totals that share the bits above; then the rows above it and, from the lowest on, as many
 // equal to it as there is room for - each warp counts a stretch of rows, and writes it behind the stretches before it.
-// The totals are read once into shared memory where they fit (44 K rows), else again in each of the five passes.
+// The ranks are held in shared memory where they fit (44 K rows), else made again in each of the five passes.
 __global__ void __launch_bounds__(ST) evict_pick(const EvictArgs A) {
     extern __shared__ uint32_t held[];
     __shared__ int hist[COPIES][BINS];
@@ -77,10 +77,10 @@ __global__ void __launch_bounds__(ST) evict_pick(const EvictArgs A) {
     }
     if (A.held) {
 #pragma unroll 8
-        for (int j = threadIdx.x; j < n; j += ST) held[j] = tot[j];
+        for (int j = threadIdx.x; j < from; j += ST) held[j] = rank_of(tot[j]);
         __syncthreads();
     }
-    auto bits = [&](int j) { return A.held ? held[j] : __ldcg(tot + j); };
+    auto rank = [&](int j) { return A.held ? held[j] : rank_of(__ldcg(tot + j)); };
     if (want > 0) {
         uint32_t prefix = 0, mask = 0;
         int left = want;  // rows still to be found among those that share `prefix`
@@ -92,7 +92,7 @@ __global__ void __launch_bounds__(ST) evict_pick(const EvictArgs A) {
             __syncthreads();
 #pragma unroll 4
             for (int j = threadIdx.x; j < from; j += ST) {
-                const uint32_t k = rank_of(bits(j));
+                const uint32_t k = rank(j);
                 if ((k & mask) == prefix) atomicAdd(&hist[lane & (COPIES - 1)][(k >> shift) & field], 1);
             }
             __syncthreads();
@@ -121,7 +121,7 @@ __global__ void __launch_bounds__(ST) evict_pick(const EvictArgs A) {
         int above = 0, equal = 0;
 #pragma unroll 4
         for (int j0 = j_lo; j0 < j_hi; j0 += 32) {
-            const uint32_t k = j0 + lane < j_hi ? rank_of(bits(j0 + lane)) : 0u;
+            const uint32_t k = j0 + lane < j_hi ? rank(j0 + lane) : 0u;
             above += __popc(__ballot_sync(0xffffffffu, j0 + lane < j_hi && k > prefix));
             equal += __popc(__ballot_sync(0xffffffffu, j0 + lane < j_hi && k == prefix));
         }
@@ -133,7 +133,7 @@ __global__ void __launch_bounds__(ST) evict_pick(const EvictArgs A) {
 #pragma unroll 4
         for (int j0 = j_lo; j0 < j_hi; j0 += 32) {
             const int j = j0 + lane;
-            const uint32_t k = j < j_hi ? rank_of(bits(j)) : 0u;
+            const uint32_t k = j < j_hi ? rank(j) : 0u;
             const unsigned eq = __ballot_sync(0xffffffffu, j < j_hi && k == prefix), below = (1u << lane) - 1u;
             const bool in = j < j_hi && (k > prefix || (k == prefix && ties + __popc(eq & below) < left));
             const unsigned kept = __ballot_sync(0xffffffffu, in);
@@ -146,7 +146,7 @@ __global__ void __launch_bounds__(ST) evict_pick(const EvictArgs A) {
     // the totals, down in order: a run is read whole before it is written (in place no later run reads what it writes)
     for (int i0 = 0; i0 < A.keep; i0 += ST) {
         const int i = i0 + threadIdx.x;
-        const uint32_t v = i < A.keep ? bits(idx[i]) : 0u;
+        const uint32_t v = i < A.keep ? __ldcg(tot + idx[i]) : 0u;
         __syncthreads();
         if (i < A.keep) tot_d[i] = v;
     }
