@@ -616,7 +616,8 @@ __global__ void __launch_bounds__(TW * 32, 1)
         const int wg = warp >> 2, row = threadIdx.x & 127;
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
         const uint32_t ts = tmem + lanes + wg * 128, to = tmem + lanes + 256 + wg * 128;
-        const float scale2 = fabsf(__fmul_rn(A.scale, LOG2E));  // (a negative scale's sign is the queries')
+        // a negative scale's sign is the queries', and a zero one's zero (a masked score stays -inf times what remains)
+        const float size2 = fabsf(__fmul_rn(A.scale, LOG2E)), scale2 = size2 == 0.f ? 1.f : size2;
         uint32_t turn = 0;  // bit b: score buffer b's phase
         uint32_t stph = 0, nph = 0;
         bool ok = true;
@@ -639,7 +640,7 @@ __global__ void __launch_bounds__(TW * 32, 1)
                         const int t = r < p.rows ? plan.order[p.order + r / G] : 0;
                         const uint4* src = reinterpret_cast<const uint4*>(A.q + ((size_t)t * A.Hq + p.head * G + r % G) * D) + x;
 #pragma unroll
-                        for (int c = 0; c < D / 64; ++c) v[i][c] = r < p.rows ? src[c * 8] : make_uint4(0u, 0u, 0u, 0u);
+                        for (int c = 0; c < D / 64; ++c) v[i][c] = r < p.rows && size2 != 0.f ? src[c * 8] : make_uint4(0u, 0u, 0u, 0u);
                     }
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {

@@ -107,13 +107,12 @@ class EvictEngine(CardEngine):
 
     # -- passes --------------------------------------------------------------------------------------------------------
     def forward(self, ids: torch.Tensor, depth: Any = None, parents: Any = None, advance: bool = True) -> torch.Tensor:
+        if depth is not None or not advance:
+            raise TypeError("rows that may be given up again would count in the totals: an evicting cache takes chains it keeps")
         T = int(ids.numel())
         self.make_room(T)
-        if depth is None:
-            depth, parents = torch.arange(T), torch.arange(-1, T - 1)
-        out = super().forward(ids, torch.as_tensor(depth, dtype=torch.int32) + self.dropped, parents, advance)
-        if advance:
-            self.rows += T
+        out = super().forward(ids, torch.arange(self.dropped, self.dropped + T, dtype=torch.int32), torch.arange(-1, T - 1))
+        self.rows += T
         return out
 
     def _attention(self, g: dict, i: int, wq: Any, wk: Any, T: int, s: int, win: int = 0, sinks: Any = None,
