@@ -815,24 +815,27 @@ __global__ void __launch_bounds__(TW * 32, 1)
                 }
             };
             int ahead[4];
-            rows_of(0, ahead);
+            if (A.tbl != nullptr) rows_of(0, ahead);
 #pragma unroll 1
             for (int i = 0; i < p.tiles && ok; ++i) {
-                int y[4];
-                bool in_line = p.keys - i * KT >= KT;
-                const int r0 = __shfl_sync(0xffffffffu, ahead[0], 0);
+                int y[4], r0 = p.start + i * KT;
+                bool box = p.keys - i * KT >= KT;  // 64 rows one after the other: one copy
+                if (A.tbl != nullptr || !box) {    // (else nothing to look up: a tile's cost here is what this warp spends on it)
+                    if (A.tbl == nullptr) rows_of(i, ahead);
+                    r0 = __shfl_sync(0xffffffffu, ahead[0], 0);
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    int r = ahead[k];
-                    in_line = in_line && r == r0 + (lane & 15) * 4 + k;
-                    if (r < 0 || r >= A.cap) {
-                        b2_fail(B2_ERR_DOMAIN);
-                        r = 0, in_line = false;
+                    for (int k = 0; k < 4; ++k) {
+                        int r = ahead[k];
+                        box = box && r == r0 + (lane & 15) * 4 + k;
+                        if (r < 0 || r >= A.cap) {
+                            b2_fail(B2_ERR_DOMAIN);
+                            r = 0, box = false;
+                        }
+                        y[k] = y0 + r;
                     }
-                    y[k] = y0 + r;
+                    box = __all_sync(0xffffffffu, box);
+                    if (A.tbl != nullptr && i + 1 < p.tiles) rows_of(i + 1, ahead);
                 }
-                const bool box = __all_sync(0xffffffffu, in_line);  // 64 rows one after the other: one copy
-                if (i + 1 < p.tiles) rows_of(i + 1, ahead);
 #pragma unroll
                 for (int kv = 0; kv < 2; ++kv) {
                     if (asked[kv] >= X.stages && !(ok = wait_or_fail(kv == 0 ? &sy.kempty[st] : &sy.vempty[st], ph, sy))) break;
