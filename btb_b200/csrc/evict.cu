@@ -43,14 +43,13 @@ __device__ __forceinline__ uint32_t rank_of(uint32_t bits) {
 
 constexpr int ST = 1024, SW = ST / 32;  // threads and warps of a selection block
 constexpr int BINS = 2048;              // eleven bits of the rank at a time: 11, 11, 10
-constexpr int COPIES = 4;               // of the histogram: many rows have equal totals, and a warp's adds to one word queue
 
 // The rank of the last kept total, eleven bits at a time from histograms of the totals that share the bits above; then the rows above it and, from the lowest on, as many
 // equal to it as there is room for - each warp counts a stretch of rows, and writes it behind the stretches before it.
-// The ranks are held in shared memory where they fit (44 K rows), else made again in each of the five passes.
+// The ranks are held in shared memory where they fit (48 K rows), else made again in each of the five passes.
 __global__ void __launch_bounds__(ST) evict_pick(const EvictArgs A) {
     extern __shared__ uint32_t held[];
-    __shared__ int hist[COPIES][BINS];
+    __shared__ int hist[BINS];
     __shared__ int sums[2][SW];
     __shared__ int s_bin, s_left;
     pdl_wait();
@@ -88,18 +87,16 @@ __global__ void __launch_bounds__(ST) evict_pick(const EvictArgs A) {
         for (int step = 0; step < 3; ++step) {
             const int shift = step == 0 ? 21 : step == 1 ? 10 : 0;
             const uint32_t field = step == 2 ? 1023u : 2047u;
-            for (int i = threadIdx.x; i < COPIES * BINS; i += ST) (&hist[0][0])[i] = 0;
+            for (int i = threadIdx.x; i < BINS; i += ST) hist[i] = 0;
             __syncthreads();
 #pragma unroll 4
             for (int j = threadIdx.x; j < from; j += ST) {
                 const uint32_t k = rank(j);
-                if ((k & mask) == prefix) atomicAdd(&hist[lane & (COPIES - 1)][(k >> shift) & field], 1);
+                if ((k & mask) == prefix) atomicAdd(&hist[(k >> shift) & field], 1);
             }
             __syncthreads();
             // thread i: bins 2047 - 2 i and the one below; how many rows lie in them and above
-            int hi = 0, lo = 0;
-#pragma unroll
-            for (int c = 0; c < COPIES; ++c) hi += hist[c][BINS - 1 - 2 * threadIdx.x], lo += hist[c][BINS - 2 - 2 * threadIdx.x];
+            const int hi = hist[BINS - 1 - 2 * threadIdx.x], lo = hist[BINS - 2 - 2 * threadIdx.x];
             int v = hi + lo;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
@@ -245,7 +242,7 @@ extern "C" int btb_b200_kv_evict(const void* K, const void* V, const void* total
                 static_cast<const int*>(n0p), static_cast<bf16*>(Kd), static_cast<bf16*>(Vd), static_cast<float*>(totals_d),
                 static_cast<int*>(n_out), static_cast<int*>(idx), static_cast<const int*>(tbl), static_cast<const int*>(tbl_d),
                 static_cast<int*>(workspace), ls, ld, hs, rs, layers, Hk, D, cap, cap_d, keep, recent, 0, 1, in_k};
-    a.held = cap <= 44 * 1024;
+    a.held = cap <= 48 * 1024;
     // in place a block for every SM, by slices of at least 64 bytes of the rows (whole rows are faster once there are enough:
     // 36 layers of 4096 rows cut to 2048 take 122 us whole, 152 in halves, 232 in quarters); else ranges of at least
     // two runs of rows
