@@ -1,5 +1,18 @@
 // Attention over long caches for sm_100a. Two entry points: btb_b200_attn_shared, a pass in the rows layout whose rows
 // share prefixes, and btb_b200_attn_scored, a chain or tree pass that also adds up what each cache row is given.
+//
+// For a row's query head q over its keys j: s_j = scale q . k_j, out = sum_j e^(s_j) v_j / (sum_j e^(s_j) + e^sink), in one pass
+// over the keys with a running maximum m and sum l of 2^(s_j log2 e - m) in f32; the weights are rounded to bf16 once, for
+// their product with the values, the sums are of the unrounded ones. A state (m, l, sum of w_j v_j) of any set of keys joins
+// another's by scaling both to the larger maximum, so the keys are cut wherever it suits the card. The totals need the
+// denominators first: w_j = 2^(s_j log2 e - m - log2 l) is made after the join, from kept scores or from the scores again.
+//
+// Launches: long_tiles (the shared prefixes on the tensor cores, the rows' own keys beside them), long_join (the states of a row
+// folded; for passes of few rows also the totals), long_weights (the totals of passes of more rows). Bound, at the largest
+// shapes, by the cache's bytes and what surrounds them: one row of 64 heads over 32768 rows of 8 kv heads (134 MB) takes 38 us a
+// call, 0.55 of the measured copy rate, 28 of them the tiles'; 32 rows over it with 128 steps of their own 47.5 us, the tiles
+// 35, the states of 256 queries a CTA (19 MB) written and folded most of the rest. Short passes (9 to 18 us) are two or three
+// launches' latencies.
 #include <cuda.h>
 
 #include <atomic>
@@ -48,7 +61,7 @@ struct LongArgs {
 // A row's own keys (its steps in the rows layout, its path in a chain or tree pass) are no one else's: units of up to
 // `chunk` keys of one (row, kv head), a warp each, beside the tiles. A one-row pass's own key joins its prefix.
 constexpr int KT = 64;         // keys a tile
-constexpr int GAP = 8;  // (4: 52.6 us where 8 takes 49.1, for 32 rows over 32768; shorter ones within 3 %)
+constexpr int GAP = 8;         // tiles (4: 52.6 us where 8 takes 49.1, for 32 rows over 32768; shorter ones within 3 %)
 constexpr int CTAS_MAX = 160;  // CTAs of the tile kernel at most
 constexpr int OWN_WARPS = 2;   // warps of a CTA that take units (two more would leave all of them 128 registers)
 
@@ -365,7 +378,7 @@ __device__ __forceinline__ uint32_t turned(uint32_t v) {  // an 8 x 8 matrix of 
 // products' k in an order of our own, the same for keys and queries. O (heads x dims) takes the weights and the values each
 // turned by movmatrix, 16 bytes of a value's row a lane. (As f32 chains, a lane a key, the units ended 4 us after the tiles of
 // 8 rows of 256 steps over a 2048-row prefix and 20 us after those of 32 rows of 128 steps over 32768: 23 and 83 us a call
-// where these take 17 and 62.) Lane 4 y + x: keys y, y + 8, ..; heads 2 x, 2 x + 1 of the
+// where these took 17 and 62.) Lane 4 y + x: keys y, y + 8, ..; heads 2 x, 2 x + 1 of the
 // scores; head y and dims 32 c + 8 x .. + 7 of the output. Keys outside are never read.
 template <int D, int G>
 __device__ __forceinline__ void own_units(const LongArgs& A, const Plan& P, int first, int stride) {
@@ -894,7 +907,9 @@ __global__ void __launch_bounds__(TW * 32, 1)
 constexpr int JT = 256, JW = JT / 32;      // threads and warps of a block
 constexpr int STATES_MAX = CTAS_MAX + 64;  // a row's parts and units
 constexpr int WEIGHT_KEYS = 4 * JT;         // keys of a block that adds up weights
-constexpr int KEEP_ROWS = 16;              // a kv head's queries (T G) up to which a pass keeps its scores for the weights
+// a kv head's queries (T G) up to which a pass keeps its scores for the weights instead of making them again. Over 32768 rows
+// of 8 heads by 8 queries, us a call kept and made again: 8 queries 37 and 54, 16 41.5 and 56, 32 51 and 59, 64 77 and 59.6
+constexpr int KEEP_ROWS = 32;
 
 // where the states of (row t, kv head g) lie: state k of query head hh in row at(k) + hh
 struct States {
@@ -955,7 +970,8 @@ __global__ void __launch_bounds__(JT) long_join(const LongArgs A, int weight_blo
         const int t = blockIdx.x / A.Hk, g = blockIdx.x - t * A.Hk, hh = warp / WH, sub = warp - hh * WH, head = g * G + hh;
         float M, L, o[E];
         // Twice: first, while the tiles are still at work, over places of the workspace whose contents are of no interest, so
-        // that the instructions are on the SM when the states are (2 us of a short pass's 10 were their first fetch).
+        // that the instructions are on the SM when the states are (two rows over 128 take 9.3 us a call so, else 9.7; one over 32768
+        // 37.4, else 38.5).
 #pragma unroll 1
         for (int real = 0; real < 2; ++real) {
             int4 a = make_int4(0, 1, 0, 1), b = make_int4(0, 1, 1, 1);
