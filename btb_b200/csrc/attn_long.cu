@@ -10,8 +10,8 @@
 // Launches: long_tiles (the shared prefixes on the tensor cores, the rows' own keys beside them), long_join (the states of a row
 // folded; for passes of few rows also the totals), long_weights (the totals of passes of more rows). Bound, at the largest
 // shapes, by the cache's bytes and what surrounds them: one row of 64 heads over 32768 rows of 8 kv heads (134 MB) takes 38 us a
-// call, 0.55 of the measured copy rate, 28 of them the tiles'; 32 rows over it with 128 steps of their own 47.5 us, the tiles
-// 35, the states of 256 queries a CTA (19 MB) written and folded most of the rest. Short passes (9 to 18 us) are two or three
+// call, 0.55 of the measured copy rate, 30 of them the tiles' (by stamps in the kernels); 32 rows over it with 128 steps of their own 47.7 us, the tiles
+// 39, the states of 256 queries a CTA (19 MB) written and folded most of the rest. Short passes (9 to 18 us) are two or three
 // launches' latencies.
 #include <cuda.h>
 
@@ -377,7 +377,7 @@ __device__ __forceinline__ uint32_t turned(uint32_t v) {  // an 8 x 8 matrix of 
 // straight from registers. S (16 keys x 8 heads) takes 16 bytes of a key's row a lane: the lane's eight dims stand for the
 // products' k in an order of our own, the same for keys and queries. O (heads x dims) takes the weights and the values each
 // turned by movmatrix, 16 bytes of a value's row a lane. (As f32 chains, a lane a key, the units ended 4 us after the tiles of
-// 8 rows of 256 steps over a 2048-row prefix and 20 us after those of 32 rows of 128 steps over 32768: 23 and 83 us a call
+// 8 rows of 256 steps over a 2048-row prefix and 20 us after those of 32 rows of 128 steps over 32768: 21 and 83 us a call
 // where these took 17 and 62.) Lane 4 y + x: keys y, y + 8, ..; heads 2 x, 2 x + 1 of the
 // scores; head y and dims 32 c + 8 x .. + 7 of the output. Keys outside are never read.
 template <int D, int G>
