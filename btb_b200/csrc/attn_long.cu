@@ -10,8 +10,9 @@
 // Launches: long_tiles (the shared prefixes on the tensor cores, the rows' own keys beside them), long_join (the states of a row
 // folded; for passes of few rows also the totals), long_weights (the totals of passes of more rows). Bound, at the largest
 // shapes, by the cache's bytes and what surrounds them: one row of 64 heads over 32768 rows of 8 kv heads (134 MB) takes 38 us a
-// call, 0.55 of the measured copy rate, 30 of them the tiles' (by stamps in the kernels); 32 rows over it with 128 steps of their own 47.7 us, the tiles
-// 39, the states of 256 queries a CTA (19 MB) written and folded most of the rest. Short passes (9 to 18 us) are two or three
+// call, 0.55 of the measured copy rate, 30 of them the tiles' (by stamps in the kernels); 32 rows over it with 128 steps of
+// their own 47.7 us, the tiles 39, the states of 256 queries a CTA (19 MB) written and folded most of the rest - in a burst at
+// 1965 MHz; run on, the power cap holds the clock near 1675 MHz and a call takes 55, its time following the clock. Short passes (9 to 18 us) are two or three
 // launches' latencies.
 #include <cuda.h>
 
