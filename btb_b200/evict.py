@@ -87,10 +87,13 @@ class EvictEngine(CardEngine):
         return g
 
     def make_room(self, T: int) -> None:
-        """evicts if the cache does not hold T more rows"""
+        """evicts if the cache does not hold T more rows; T that it would not hold even then are refused, and nothing leaves"""
         if self.dropped + self.rows + T > self.positions:
             raise ValueError(f"position {self.dropped + self.rows + T} of {self.positions}")
         if self.rows + T > self.cap:
+            stay = min(self.rows, self.keep)
+            if stay + T > self.cap:
+                raise ValueError(f"{T} rows beside the {stay} that stay in a cache of {self.cap}")
             self.evict()
 
     def evict(self) -> None:
