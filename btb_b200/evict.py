@@ -17,7 +17,7 @@ import torch
 
 from . import capi
 from .capi import ptr
-from .engine import CardEngine, ModelWeights, rope_tables
+from .engine import CardEngine, ModelWeights, pad_rows, rope_tables
 
 PASS_ROWS = 32  # rows a pass at most
 
@@ -113,6 +113,7 @@ class EvictEngine(CardEngine):
         if depth is not None or not advance:
             raise TypeError("rows that may be given up again would count in the totals: an evicting cache takes chains it keeps")
         T = int(ids.numel())
+        pad_rows(T)  # (more rows than a pass holds are refused before any leave)
         self.make_room(T)
         out = super().forward(ids, torch.arange(self.dropped, self.dropped + T, dtype=torch.int32), torch.arange(-1, T - 1))
         self.rows += T

@@ -4,7 +4,7 @@ anything has moved."""
 import pytest
 import torch
 
-from btb_b200.engine import CardEngine
+from btb_b200.engine import CardEngine, pad_rows
 from btb_b200.evict import EvictEngine
 
 
@@ -18,7 +18,7 @@ def bare(monkeypatch, rows, budget=160, keep=64, positions=2048):
             e.dropped, e.rows, e.cuts = e.dropped + e.rows - e.keep, e.keep, e.cuts + 1
 
     e.evict = evict
-    monkeypatch.setattr(CardEngine, "forward", lambda self, ids, depth, parents: torch.zeros(int(ids.numel()), 4))
+    monkeypatch.setattr(CardEngine, "forward", lambda self, ids, depth, parents: torch.zeros(pad_rows(int(ids.numel())), 4))
     return e
 
 
@@ -51,3 +51,12 @@ def test_a_graph_of_more_steps_than_fit_is_refused_at_its_replay_too(monkeypatch
     with pytest.raises(ValueError):
         steps.replay()
     assert g.replays == 1 and (e.rows, e.dropped, e.cuts) == (100, 0, 0)
+
+
+def test_a_pass_of_too_many_rows_lets_none_go(monkeypatch):
+    e = bare(monkeypatch, 160)
+    with pytest.raises(ValueError):
+        e.forward(torch.arange(33))
+    assert (e.rows, e.dropped, e.cuts) == (160, 0, 0)
+    e.forward(torch.arange(32))
+    assert (e.rows, e.dropped, e.cuts) == (96, 96, 1)
