@@ -39,6 +39,8 @@ class EvictEngine(CardEngine):
     Until the first eviction its tokens are the engine's own, to the attention's rounding. `positions`: the longest
     conversation, in tokens (rows of the rotary tables)."""
 
+    evicts = True  # rows of the cache may leave it: no `Session` stands over it
+
     def __init__(self, weights: ModelWeights, budget: int = 4096, keep: int | None = None, recent: int | None = None,
                  positions: int | None = None, device: Any = "cuda"):  # fmt: skip
         keep = int(budget) // 2 if keep is None else int(keep)
@@ -145,9 +147,6 @@ class EvictEngine(CardEngine):
     # -- what a cache that rows leave cannot do --------------------------------------------------------------------------
     def prefill_gemm(self, prompt: torch.Tensor, chunk: int = 256) -> torch.Tensor:
         raise TypeError("prefill_gemm's attention adds up no totals: an evicting cache is filled by prefill")
-
-    def session(self) -> Any:
-        raise TypeError("a session goes back to earlier rows, and an evicting cache may have let them go")
 
     def generate_speculative(self, prompt: Any, max_new: int, budget: int = 8, v_max: int = 8) -> tuple[list[int], dict]:
         raise TypeError("a verify pass's rejected rows would count in the totals: no speculation over an evicting cache")

@@ -49,6 +49,8 @@ class Session:
     CHUNK = 32  # rows a pass carries at most (btb/engine/cuda.py CARD_T_MAX)
 
     def __init__(self, engine: Any) -> None:
+        if getattr(engine, "evicts", False):
+            raise TypeError("a session goes back to earlier rows, and an evicting cache may have let them go")
         self.engine = engine
         self.ids: list[int] = []  # the tokens whose rows stand in the cache
         self.n_prompt = 0

@@ -6,6 +6,7 @@ import torch
 
 from btb_b200.engine import CardEngine, pad_rows
 from btb_b200.evict import EvictEngine
+from btb_b200.session import Session
 
 
 def bare(monkeypatch, rows, budget=160, keep=64, positions=2048):
@@ -60,3 +61,11 @@ def test_a_pass_of_too_many_rows_lets_none_go(monkeypatch):
     assert (e.rows, e.dropped, e.cuts) == (160, 0, 0)
     e.forward(torch.arange(32))
     assert (e.rows, e.dropped, e.cuts) == (96, 96, 1)
+
+
+def test_a_session_over_it_is_refused_however_it_is_made(monkeypatch):
+    """a session moves the cache's length by itself, and goes back to rows that may have left"""
+    e = bare(monkeypatch, 0)
+    for make in (e.session, lambda: Session(e)):
+        with pytest.raises(TypeError):
+            make()
