@@ -138,6 +138,9 @@ class RowsEngine(CardEngine):
     instead of once a row. A row then agrees with its own decode to rounding, not to the bit."""
 
     def __init__(self, weights: ModelWeights, cap: int = 4096, device: Any = "cuda", shared: bool = False):
+        c = weights.cfg
+        if shared and not int(capi.lib().btb_b200_attn_shared_workspace_bytes(32, c.q_heads, c.kv_heads, c.head_dim)):
+            raise ValueError(f"{c.q_heads} query heads over {c.kv_heads} kv heads of {c.head_dim}: no shared attention for them")
         super().__init__(weights, cap=cap, step_kernel=False, device=device)
         self.shared = bool(shared)
         self._shared_ws: Any = None
