@@ -184,19 +184,28 @@ __global__ void __launch_bounds__(MT) evict_move(const EvictArgs A) {
     };
     int ahead[MC];
     uint4 next[MC];
+    unsigned has = 0;  // bit c: piece c of the next run has a source (a row past the end or outside the cache has none, and is not written)
 #pragma unroll
     for (int c = 0; c < MC; ++c) ahead[c] = from(lo + c * rows + row);
 #pragma unroll
-    for (int c = 0; c < MC; ++c) next[c] = ahead[c] >= 0 ? src[ahead[c] * rs] : make_uint4(0u, 0u, 0u, 0u);
+    for (int c = 0; c < MC; ++c) {
+        next[c] = ahead[c] >= 0 ? src[ahead[c] * rs] : make_uint4(0u, 0u, 0u, 0u);
+        has |= (unsigned)(ahead[c] >= 0) << c;
+    }
 #pragma unroll
     for (int c = 0; c < MC; ++c) ahead[c] = from(lo + run + c * rows + row);
 #pragma unroll 1
     for (int i0 = lo; i0 < hi; i0 += run) {
         uint4 v[MC];
+        const unsigned here = has;
+        has = 0;
 #pragma unroll
         for (int c = 0; c < MC; ++c) v[c] = next[c];
 #pragma unroll
-        for (int c = 0; c < MC; ++c) next[c] = ahead[c] >= 0 ? src[ahead[c] * rs] : make_uint4(0u, 0u, 0u, 0u);
+        for (int c = 0; c < MC; ++c) {
+            next[c] = ahead[c] >= 0 ? src[ahead[c] * rs] : make_uint4(0u, 0u, 0u, 0u);
+            has |= (unsigned)(ahead[c] >= 0) << c;
+        }
 #pragma unroll
         for (int c = 0; c < MC; ++c) ahead[c] = from(i0 + 2 * run + c * rows + row);
         if (A.in_place) {
@@ -207,7 +216,7 @@ __global__ void __launch_bounds__(MT) evict_move(const EvictArgs A) {
 #pragma unroll
         for (int c = 0; c < MC; ++c) {
             const int i = i0 + c * rows + row;
-            if (!on || i >= hi) continue;
+            if (!(here >> c & 1u)) continue;
             const int r = A.tbl_d != nullptr ? A.tbl_d[i] : i;
             if (r < 0 || r >= A.cap_d) b2_fail(B2_ERR_DOMAIN);
             else dst[r * rs] = v[c];

@@ -213,7 +213,9 @@ size_t btb_b200_attn_scored_workspace_bytes(int T, int Hq, int Hk, int D, int ca
  * [layers, Hk, cap], totals_d [layers, Hk, cap_d]; idx i32 [layers, Hk, keep] gets the kept rows' old numbers (-1 past the
  * count), n_out the count (may be n0p's own word: the rest of the cache then stands after it). Rows past the count are
  * left as they were. tbl, tbl_d: logical row -> cache row of source and destination, or null. D a multiple of 8;
- * 0 <= recent <= keep <= cap_d. A count outside the cache writes nothing but the status word. workspace: btb_b200_kv_evict_workspace_bytes bytes, 16-byte aligned, no contents needed. */
+ * 0 <= recent <= keep <= cap_d. A count outside the cache writes nothing but the status
+ * word; a kept row whose map entry lies outside its cache is not moved (the status word; its place stays as it was).
+ * workspace: btb_b200_kv_evict_workspace_bytes bytes, 16-byte aligned, no contents needed. */
 int btb_b200_kv_evict(const void* K, const void* V, const void* totals, const void* n0p, void* Kd, void* Vd,
                       void* totals_d, void* n_out, void* idx, int layers, long long ls, long long ld, int Hk, int D,
                       long long hs, long long rs, int cap, int cap_d, int keep, int recent, const void* tbl,
