@@ -1274,9 +1274,10 @@ int launch(void (*kern)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t 
 }
 
 int long_ctas() { return min(b2_sm_count(), CTAS_MAX); }
-// rows of the parts at most: every CTA's stretch moves on by one item's rows, every kv head by its items'
-size_t part_rows(int T, int Hq) { return (size_t)long_ctas() * T * Hq + (size_t)T * Hq; }
-size_t state_rows(int T, int Hq, int Hk) { return part_rows(T, Hq) + (size_t)T * Hq * units_max(T, Hk); }
+// rows of the parts at most: a CTA's stretch moves on by the rows of a kv head's items, T G at most, and a kv head by as many
+// (32 rows of 64 heads over 8 kv heads of 128: 38 MB with the units' rows)
+size_t part_rows(int T, int Hq, int Hk) { return (size_t)long_ctas() * T * (Hq / Hk) + (size_t)T * Hq; }
+size_t state_rows(int T, int Hq, int Hk) { return part_rows(T, Hq, Hk) + (size_t)T * Hq * units_max(T, Hk); }
 constexpr size_t INFO_BYTES = TMAX * 2 * sizeof(int4);
 long long score_stride(int cap) { return ((long long)cap + KT - 1) / KT * KT; }
 bool keeps_scores(int T, int Hq, int Hk) { return T * (Hq / Hk) <= KEEP_ROWS; }
@@ -1350,7 +1351,7 @@ static float* take_states(LongArgs& a, void* workspace, int D) {
     a.info = static_cast<int4*>(workspace);
     a.part_o = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + INFO_BYTES);
     a.part_ml = reinterpret_cast<float2*>(a.part_o + rows * D);
-    a.unit_row = (long long)part_rows(a.T, a.Hq);
+    a.unit_row = (long long)part_rows(a.T, a.Hq, a.Hk);
     return reinterpret_cast<float*>(a.part_ml + rows);
 }
 

@@ -165,3 +165,32 @@ def test_prefixes_of_uneven_rows(of, lens, D, Hk):
     got = shared(q, K, V, hs, rs, lay, cap)
     check_shared(q, K, V, lay, got, 32)
     assert torch.equal(shared(q, K, V, hs, rs, lay, cap), got) and capi.status() == 0
+
+
+# ---- the workspace --------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("T,Hq,Hk,D,n", [(32, 64, 8, 128, 20000), (32, 8, 8, 64, 9000), (1, 8, 1, 128, 30000), (3, 256, 32, 64, 4000),
+                                         (17, 16, 2, 128, 700), (4, 200, 200, 64, 300)])  # fmt: skip
+@pytest.mark.parametrize("prefixes", [1, 5])
+def test_nothing_is_written_behind_a_workspace(T, Hq, Hk, D, n, prefixes):
+    g = gen(n + T)
+    lens = [max(1, n - 64 * p) // min(prefixes, T) for p in range(min(prefixes, T))]
+    offs = [sum(lens[:p]) for p in range(len(lens))]
+    base, step = sum(lens), 40
+    cap = base + (step + 1) * T
+    lay = [base, step, T]
+    for t in range(T):
+        lay += [t, offs[t % len(lens)], lens[t % len(lens)]]
+    K, V, hs, rs = cache(g, cap, Hk, D)
+    q = torch.randn(T, Hq, D, generator=g, device=DEV).to(BF)
+    guard = 1 << 18  # words of a pattern behind it
+    for name, dims in (("shared", (T, Hq, Hk, D)), ("scored", (T, Hq, Hk, D, cap))):
+        size = int(getattr(capi.lib(), f"btb_b200_attn_{name}_workspace_bytes")(*dims))
+        ws = torch.full(((size + 3) // 4 + guard,), 0x5A5A5A5A, dtype=torch.int32, device=DEV)
+        if name == "shared":
+            check_shared(q, K, V, lay, shared(q, K, V, hs, rs, lay, cap, ws=ws), T)
+        else:
+            totals = torch.zeros(Hk, cap, device=DEV)
+            got = scored(q, K, V, hs, rs, base, chain(T), totals, cap, ws=ws)
+            check_scored(q, K, V, base, chain(T), torch.zeros_like(totals), got, totals)
+        assert bool((ws[-guard:] == 0x5A5A5A5A).all()), name
+    assert capi.status() == 0
