@@ -614,9 +614,11 @@ __global__ void __launch_bounds__(TW * 32, 1)
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
         tm_before();
     }
-    // the kernels before are through; only now may the joining kernel start, which reads what they left before it waits
+    // The kernels before are through; only now may the joining kernel start, which reads what they left before it waits. The warp
+    // that took the tensor memory says so: no kernel that starts on it can take tensor memory ahead of this CTA, and then wait
+    // for this CTA while this CTA waits for it.
     pdl_wait();
-    pdl_launch_dependents();
+    if (warp == 9) pdl_launch_dependents();
     if (warp == 0) make_plan<G>(A, plan, blockIdx.x == 0);
     __syncthreads();
     const Cut cut(plan.line * A.Hk, gridDim.x);

@@ -194,3 +194,49 @@ def test_nothing_is_written_behind_a_workspace(T, Hq, Hk, D, n, prefixes):
             check_scored(q, K, V, base, chain(T), torch.zeros_like(totals), got, totals)
         assert bool((ws[-guard:] == 0x5A5A5A5A).all()), name
     assert capi.status() == 0
+
+
+def test_two_streams_of_passes_and_tensor_core_matvecs():
+    """on each of two streams a pass of totals (three launches), a shared pass and a tensor-core matvec of its output, all of which
+    take tensor memory and start under programmatic launch, over and over beside one another: the bits of a run alone"""
+    runs = []
+    for D, Hq, Hk, T, n in ((64, 32, 4, 16, 900), (128, 16, 2, 32, 1500)):
+        g = gen(D)
+        lay, cap = [n, 9, T], n + 10 * T
+        for t in range(T):
+            lay += [t, 0, n]
+        K, V, hs, rs = cache(g, cap, Hk, D)
+        q = torch.randn(T, Hq, D, generator=g, device=DEV).to(BF)
+        R, C = 2048, Hq * D
+        W = (torch.randn(R, C, generator=g, device=DEV) / C**0.5).to(BF)
+        rw = torch.tensor(lay, dtype=torch.int32, device=DEV)
+        n0, par = torch.tensor([n], dtype=torch.int32, device=DEV), torch.tensor(tree(T), dtype=torch.int32, device=DEV)
+        wss = [workspace("btb_b200_attn_shared_workspace_bytes", T, Hq, Hk, D), workspace("btb_b200_attn_scored_workspace_bytes", T, Hq, Hk, D, cap)]
+        wtc = torch.zeros(max(4, int(capi.lib().btb_b200_gemv_tc_workspace_bytes(R, C)) // 4), dtype=torch.float32, device=DEV)
+        assert not keeps_scores(T, Hq, Hk, D)
+
+        def go(q=q, K=K, V=V, hs=hs, rs=rs, rw=rw, n0=n0, par=par, cap=cap, wss=wss, wtc=wtc, W=W, R=R, C=C, T=T, Hk=Hk):
+            outs = [torch.empty(T, C, dtype=BF, device=DEV) for _ in range(2)]
+            y, totals = torch.empty(2, T, R, dtype=BF, device=DEV), torch.zeros(Hk, cap, device=DEV)
+            for i in range(2):
+                if i == 0:
+                    scored(q, K, V, hs, rs, n0, par, totals, cap, out=outs[0], ws=wss[1])
+                else:
+                    shared(q, K, V, hs, rs, rw, cap, out=outs[1], ws=wss[0])
+                call("btb_b200_gemv_tc_bf16", ptr(W), ptr(outs[i]), ptr(y[i]), T, R, C, ptr(wtc), capi.stream_ptr())
+            return outs[0], outs[1], y, totals
+
+        want = go()
+        torch.cuda.synchronize()
+        runs.append((go, want))
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [[], []]
+    for _ in range(25):
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(runs[i][0]())
+    torch.cuda.synchronize()
+    for i in range(2):
+        for outs in got[i]:
+            assert all(torch.equal(a, b) for a, b in zip(outs, runs[i][1]))
+    assert capi.status() == 0
