@@ -135,7 +135,11 @@ class RowsEngine(CardEngine):
     A row reads its keys in logical order, so its bits are its own one-sequence decode's whatever rows step beside it.
 
     `shared`: the attention goes over a prefix that several rows share once for all of them (`btb_b200_attn_shared`)
-    instead of once a row. A row then agrees with its own decode to rounding, not to the bit."""
+    instead of once a row. A row then agrees with its own decode to rounding, not to the bit. It pays from a few hundred rows
+    of prefix on, the more rows share it the more: a step of the 4 B dense model (`wide_tc`, the 61st after the fork) over 2048
+    rows takes 2.36 ms instead of 2.70 for two forks and 3.67 instead of 6.37 for 32; over 128 rows 2.27 instead of 2.32 and
+    3.52 instead of 3.81. The attention kernels alone are the slower ones there for up to eight rows: by 0.4 to 1.5 us for 32
+    heads over 8, by 3 to 4 where every query head has a kv head of its own."""
 
     def __init__(self, weights: ModelWeights, cap: int = 4096, device: Any = "cuda", shared: bool = False):
         c = weights.cfg

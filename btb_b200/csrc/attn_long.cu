@@ -10,10 +10,12 @@
 // Launches: long_tiles (the shared prefixes on the tensor cores, the rows' own keys beside them), long_join (the states of a row
 // folded; for passes of few rows also the totals), long_weights (the totals of passes of more rows). Bound, at the largest
 // shapes, by the cache's bytes and what surrounds them: one row of 64 heads over 32768 rows of 8 kv heads (134 MB) takes 38 us a
-// call, 0.55 of the measured copy rate, 30 of them the tiles' (by stamps in the kernels); 32 rows over it with 128 steps of
-// their own 47.7 us, the tiles 39, the states of 256 queries a CTA (19 MB) written and folded most of the rest - in a burst at
-// 1965 MHz; run on, the power cap holds the clock near 1675 MHz and a call takes 55, its time following the clock. Short passes (9 to 18 us) are two or three
-// launches' latencies.
+// call, 0.55 of the measured copy rate; by stamps in the kernels its CTAs end their tiles 25 to 33 us after they began, half of
+// them by 31, and all wait for the last. 32 rows over it with 128 steps of their own take 47.7 us, the CTAs' tiles 32 to 43,
+// half by 39.5, the states of 256 queries a CTA (19 MB) written and folded most of the rest - in a burst at 1965 MHz; run on, the
+// power cap holds the clock near 1675 MHz and a call takes 55, its time following the clock. Short passes (9 to 18 us) are two
+// or three launches' latencies. btb_b200_attn_decode_rows takes 98 us and 1981 for those rows (63 steps of their own); it is
+// the faster one below a few hundred keys (eight rows of 8 heads over 8 kv heads, 128 keys: 6.1 us against 10.5).
 #include <cuda.h>
 
 #include <atomic>
@@ -911,7 +913,8 @@ constexpr int JT = 256, JW = JT / 32;      // threads and warps of a block
 constexpr int STATES_MAX = CTAS_MAX + 64;  // a row's parts and units
 constexpr int WEIGHT_KEYS = 4 * JT;         // keys of a block that adds up weights
 // a kv head's queries (T G) up to which a pass keeps its scores for the weights instead of making them again. Over 32768 rows
-// of 8 heads by 8 queries, us a call kept and made again: 8 queries 37 and 54, 16 41.5 and 56, 32 51 and 59, 64 77 and 59.6
+// of 8 heads by 8 queries, us a call kept and made again: 8 queries 37 and 54, 16 41.5 and 56, 32 51 and 59, 64 77 and 59.6. (That
+// length alone was measured: shorter caches, whose scores are fewer bytes, go by the same number.)
 constexpr int KEEP_ROWS = 32;
 
 // where the states of (row t, kv head g) lie: state k of query head hh in row at(k) + hh
@@ -1310,7 +1313,9 @@ int launch_long(const LongArgs& a, cudaStream_t s) {
     if (a.totals == nullptr || a.scores != nullptr) return B2_OK;
     auto weights = long_weights<D>;
     if (const int rc = b2_allow_smem(reinterpret_cast<const void*>(weights), weights_allowed)) return rc;
-    const int N = (a.T * G + 31) & ~31;  // two blocks an SM
+    // a grid of two blocks an SM. (Nothing holds an SM to two: at head dim 64 its shared memory has room for four, and of more
+    // than 512 columns of tensor memory the later blocks wait until the earlier ones have ended)
+    const int N = (a.T * G + 31) & ~31;
     return launch(weights, dim3(min((a.cap + WT - 1) / WT, max(1, 2 * a.ctas / a.Hk)), a.Hk), dim3(WT), (size_t)(WT + N) * D * 2, s, tm[0], tm[1], x);
 }
 template <int D>

